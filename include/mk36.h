@@ -418,6 +418,117 @@ MK36_API size_t mk36_linear_workspace_bytes(const mk36_linear_args* args);
 MK36_API int mk36_linear_decode(const mk36_linear_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * A paged KV cache held in 4 bits, with sequences of different lengths.
+ *
+ * No counterpart among the reference's kernels: its decode task graph names a `paged_attention` task
+ * (mega_kernel_qwen36/mpk_graph.py:352-398) and leaves it to the caller; its operator takes dense caches of one length
+ * (mega_kernel_qwen36/reference.py:117-145).
+ *
+ * Cache: pool, bytes [pages][kv_heads][page_size / 16][tile_bytes], 16-byte aligned, tile_bytes = head_dim * (16 +
+ * element size of dtype).  A tile holds 16 consecutive tokens of one KV head: key codes (8 head_dim bytes), value codes,
+ * key parameters, value parameters.  A group of 64 channels of a token has a scale and a zero point in `dtype`
+ * (parameters: [16][head_dim / 64]{scale, zero}); an entry stands for zero + code * scale with a code of 0 .. 15.  With
+ * i, the place of the half byte in a little-endian 32-bit word, = channel % 8, the word of token t, channel c lies at
+ *   keys:   ((t / 8) * (D / 8 / u) + b / u) * 32 u + ((t % 8) * 4 + (c % 64) / 16) * u + b % u,
+ *           b = c / 64 * 8 + (c % 16) / 8 * 4,  u = min(16, D / 8)
+ *   values: (t % 2 + 2 (t / 8)) * 2 D + ((c % 64) / 8 * 4 + (t % 8) / 2) * (D / 16) + c / 64 * 4
+ * of its codes.  page_size is a multiple of 16; head_dim 64, 128 or 256.
+ *
+ * page_table int32 [rows, row_pages]: page of each page_size tokens of a row, -1 where it has none; lengths int32 [rows].
+ * Both are read on the device: no call waits for the host, and captured calls follow what the tables hold at replay.
+ * Lengths below zero count as zero, lengths beyond row_pages * page_size as that.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct mk36_kv4_cache {
+    void* pool;
+    const int32_t* page_table;
+    const int32_t* lengths;
+    int64_t pages;
+    int32_t dtype; /* of keys, values, queries, outputs and parameters */
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t page_size;
+    int32_t rows;
+    int32_t row_pages;
+} mk36_kv4_cache;
+
+/* Keys and values of the LAST tokens of every row, k and v [rows, tokens, kv_heads, head_dim]; with cu_tokens (int32
+ * [rows + 1], ascending from 0) [tokens, kv_heads, head_dim], row r having the tokens cu_tokens[r] .. cu_tokens[r + 1] - 1.
+ * A row's n tokens are its positions lengths[r] - n .. lengths[r] - 1: lengths already count what is appended.  Strides are
+ * in elements (k_row and v_row are not used with cu_tokens), the channels contiguous. */
+typedef struct mk36_kv4_tokens {
+    void* k;
+    void* v;
+    const int32_t* cu_tokens;
+    int64_t tokens; /* of each row, or of all rows with cu_tokens */
+    int64_t k_row, k_token, k_head;
+    int64_t v_row, v_token, v_head;
+} mk36_kv4_tokens;
+
+/* Quantises and writes them.  Of a group: zero = the least value, scale = (greatest - least) / 15 rounded to dtype, code =
+ * (value - zero) / scale rounded to the nearest (halves to even), at most 15, all of it exact before each rounding; codes are 0 where
+ * the scale is 0.  A group with an infinity or a NaN stands for NaN.  Tokens without a place (position below zero, no page or one
+ * outside the pool, behind the last row) are not written.  No two rows may hold the page that a token is written to. */
+MK36_API int mk36_kv4_append(const mk36_kv4_cache* cache, const mk36_kv4_tokens* tokens, void* stream);
+/* Reads them back, rounded once; tokens of a position below zero come back as zeros, those without a page in the pool as NaN, and
+ * what lies behind the last row's tokens is left as it was. */
+MK36_API int mk36_kv4_read(const mk36_kv4_cache* cache, const mk36_kv4_tokens* tokens, void* stream);
+
+/* Attention of the last `tokens` tokens of every row over the row: q, out [rows, tokens, query_heads, head_dim] (out dense, q
+ * with strides in elements and contiguous channels), token i of a row sees the positions 0 .. lengths[r] - tokens + i.  A
+ * query that sees nothing gives zeros; one that reaches a page outside the pool gives NaN.  The workspace is scratch for this call
+ * alone (it need not be initialised): two calls that may overlap, or two captured graphs, have one each. */
+typedef struct mk36_kv4_attention_args {
+    const void* q;
+    void* out;
+    int64_t q_row, q_token, q_head;
+    int32_t query_heads;
+    int32_t tokens;
+    float scale;
+} mk36_kv4_attention_args;
+
+MK36_API size_t mk36_kv4_attention_workspace_bytes(const mk36_kv4_cache* cache, const mk36_kv4_attention_args* args);
+MK36_API int mk36_kv4_attention_decode(const mk36_kv4_cache* cache, const mk36_kv4_attention_args* args, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/* Upkeep of the tables.  refcounts int32 [pages]: rows that hold the page; a page with 0 is free.  Every call takes the tables
+ * as *_in and gives them as *_out, which may be the same arrays.  Results do not depend on the order of threads.  *status
+ * (device) says how it went; where it is not 0 (fork, resize) the tables come out as they went in and no page is written.
+ *   fork    row children[i] becomes a copy of row parents[i] that shares its pages (every entry >= 0), i < count.  Pairs with a
+ *           negative index are skipped.  Status -1: an index beyond the rows, a child that is not empty or that comes twice.
+ *   resize  row r goes from lengths[r] to new_lengths[r] tokens.  Pages behind its new end lose a reference and its entries become
+ *           -1; then a row that grows, and whose last page is filled in part and shared, gets a copy of it (the tiles that hold tokens), and
+ *           new pages are taken, lowest free number first, in the order of rows and, in a row, the copy first.  Status n > 0: n pages
+ *           are missing; -1: a length below 0 or beyond row_pages * page_size, or an entry outside the pool where a page is held.
+ *   compact pages in use behind the first n, n the number of pages in use, move to the free ones among the first n, both
+ *           ascending; *status = n.
+ * pool, kv_heads, page_size and tile_bytes are those of the cache (resize, compact). */
+typedef struct mk36_kv_pages_args {
+    const int32_t* page_table_in;
+    const int32_t* lengths_in;
+    const int32_t* refcounts_in;
+    int32_t* page_table_out;
+    int32_t* lengths_out;
+    int32_t* refcounts_out;
+    int32_t* status;
+    void* pool;
+    const int32_t* new_lengths; /* resize [rows] */
+    const int32_t* parents;     /* fork [count] */
+    const int32_t* children;
+    int64_t pages;
+    int32_t rows;
+    int32_t row_pages;
+    int32_t count;
+    int32_t kv_heads;
+    int32_t page_size;
+    int32_t tile_bytes;
+} mk36_kv_pages_args;
+
+MK36_API size_t mk36_kv_pages_workspace_bytes(const mk36_kv_pages_args* args);
+MK36_API int mk36_kv_pages_fork(const mk36_kv_pages_args* args, void* workspace, size_t workspace_bytes, void* stream);
+MK36_API int mk36_kv_pages_resize(const mk36_kv_pages_args* args, void* workspace, size_t workspace_bytes, void* stream);
+MK36_API int mk36_kv_pages_compact(const mk36_kv_pages_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Multi-GPU (one process per GPU, all GPUs on one NVLink / NVSwitch box).
  *
  * The reference is single-GPU; these entry points have no counterpart there.  They run the same

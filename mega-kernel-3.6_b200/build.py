@@ -46,6 +46,9 @@ CUDA_SOURCES = [
     "attention_decode_static.cu",
     "linear_attention_decode.cu",
     "linear_decode.cu",
+    "kv4_tokens.cu",
+    "kv4_attention.cu",
+    "kv_pages.cu",
 ]
 LIB_NAME = "libmk36.so"
 

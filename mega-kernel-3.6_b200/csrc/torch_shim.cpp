@@ -601,6 +601,196 @@ std::tuple<torch::Tensor, torch::Tensor> linear_attention_decode_steps(torch::Te
     return std::make_tuple(out, new_state);
 }
 
+// -------------------------------------------------------------------------------------------
+// The 4-bit paged cache.  Scratch is taken from the allocator for each call, on the current stream: calls on other streams
+// and captured graphs share none.
+// -------------------------------------------------------------------------------------------
+void check_int_table(const torch::Tensor& t, const torch::Tensor& like, const char* name, int64_t dims) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.device() == like.device(), name, " must be on the device of the pool");
+    TORCH_CHECK(t.scalar_type() == torch::kInt32, name, " must be int32");
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+    TORCH_CHECK(t.dim() == dims, name, " must have ", dims, " dimension(s)");
+}
+
+mk36_kv4_cache kv4_cache(const torch::Tensor& pool, const torch::Tensor& pages, const torch::Tensor& lengths, int64_t head_dim,
+                         torch::ScalarType dtype) {
+    SHIM_CHECK_INPUT(pool);
+    TORCH_CHECK(pool.scalar_type() == torch::kUInt8 && pool.dim() == 4, "pool must be uint8 [pages, kv_heads, page_size / 16, tile_bytes]");
+    check_int_table(pages, pool, "pages", 2);
+    check_int_table(lengths, pool, "lengths", 1);
+    TORCH_CHECK(lengths.size(0) == pages.size(0), "lengths must have an entry for each row of pages");
+    const torch::Tensor like = torch::empty({0}, torch::TensorOptions().dtype(dtype));
+    mk36_kv4_cache c{};
+    c.dtype = dtype_code(like, "kv4 cache");
+    TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256");
+    TORCH_CHECK(pool.size(3) == head_dim * (16 + static_cast<int64_t>(like.element_size())), "pool has tiles of ", pool.size(3), " bytes, head_dim ",
+                head_dim, " in ", dtype, " takes ", head_dim * (16 + static_cast<int64_t>(like.element_size())));
+    TORCH_CHECK(pool.size(2) * 16 <= 0x7fffffff && pool.size(1) <= 0x7fffffff && pages.size(0) <= 0x7fffffff && pages.size(1) <= 0x7fffffff,
+                "pool or pages has a dimension beyond 32 bits");
+    c.pool = pool.data_ptr();
+    c.page_table = pages.data_ptr<int32_t>();
+    c.lengths = lengths.data_ptr<int32_t>();
+    c.pages = pool.size(0);
+    c.kv_heads = static_cast<int32_t>(pool.size(1));
+    c.head_dim = static_cast<int32_t>(head_dim);
+    c.page_size = static_cast<int32_t>(pool.size(2) * 16);
+    c.rows = static_cast<int32_t>(pages.size(0));
+    c.row_pages = static_cast<int32_t>(pages.size(1));
+    return c;
+}
+
+mk36_kv4_tokens kv4_tokens(const mk36_kv4_cache& c, const torch::Tensor& pool, const torch::Tensor& k, const torch::Tensor& v,
+                           const std::optional<torch::Tensor>& cu_tokens) {
+    mk36_kv4_tokens t{};
+    const bool ragged = cu_tokens.has_value();
+    for (const torch::Tensor* x : {&k, &v}) {
+        const char* name = x == &k ? "k" : "v";
+        TORCH_CHECK(x->is_cuda() && x->device() == pool.device(), name, " must be on the device of the pool");
+        TORCH_CHECK(dtype_code(*x, "kv4") == c.dtype, name, " and cache dtype mismatch");
+        if (ragged) {
+            TORCH_CHECK(x->dim() == 3, name, " must be [tokens, kv_heads, head_dim] with cu_tokens");
+        } else {
+            TORCH_CHECK(x->dim() == 4 && x->size(0) == c.rows, name, " must be [rows, tokens, kv_heads, head_dim]");
+        }
+        TORCH_CHECK(x->size(-2) == c.kv_heads && x->size(-1) == c.head_dim, name, " must have the cache's kv_heads and head_dim");
+        TORCH_CHECK(x->stride(-1) == 1, name, " must have contiguous channels");
+    }
+    TORCH_CHECK(v.sizes() == k.sizes(), "v shape must match k");
+    if (ragged) {
+        check_int_table(*cu_tokens, pool, "cu_tokens", 1);
+        TORCH_CHECK(cu_tokens->size(0) == c.rows + 1, "cu_tokens must have rows + 1 entries");
+        t.cu_tokens = cu_tokens->data_ptr<int32_t>();
+    }
+    t.k = k.data_ptr();
+    t.v = v.data_ptr();
+    t.tokens = k.size(ragged ? 0 : 1);
+    if (!ragged) t.k_row = k.stride(0), t.v_row = v.stride(0);
+    t.k_token = k.stride(-3), t.k_head = k.stride(-2);
+    t.v_token = v.stride(-3), t.v_head = v.stride(-2);
+    return t;
+}
+
+void kv4_append(torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, int64_t head_dim, torch::Tensor k, torch::Tensor v,
+                std::optional<torch::Tensor> cu_tokens) {
+    const mk36_kv4_cache c = kv4_cache(pool, pages, lengths, head_dim, k.scalar_type());
+    const mk36_kv4_tokens t = kv4_tokens(c, pool, k, v, cu_tokens);
+    const c10::cuda::CUDAGuard guard(pool.device());
+    pool.unsafeGetTensorImpl()->bump_version();
+    check_rc(mk36_kv4_append(&c, &t, at::cuda::getCurrentCUDAStream().stream()));
+}
+
+void kv4_read(torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, int64_t head_dim, torch::Tensor k, torch::Tensor v,
+              std::optional<torch::Tensor> cu_tokens) {
+    const mk36_kv4_cache c = kv4_cache(pool, pages, lengths, head_dim, k.scalar_type());
+    const mk36_kv4_tokens t = kv4_tokens(c, pool, k, v, cu_tokens);
+    const c10::cuda::CUDAGuard guard(pool.device());
+    k.unsafeGetTensorImpl()->bump_version();
+    v.unsafeGetTensorImpl()->bump_version();
+    check_rc(mk36_kv4_read(&c, &t, at::cuda::getCurrentCUDAStream().stream()));
+}
+
+torch::Tensor kv4_attention_decode(torch::Tensor q, torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, int64_t head_dim, double scale) {
+    const mk36_kv4_cache c = kv4_cache(pool, pages, lengths, head_dim, q.scalar_type());
+    TORCH_CHECK(q.is_cuda() && q.device() == pool.device(), "q must be on the device of the pool");
+    TORCH_CHECK((q.dim() == 3 || q.dim() == 4) && q.size(0) == c.rows, "q must be [rows, query_heads, head_dim] or [rows, tokens, query_heads, head_dim]");
+    TORCH_CHECK(q.size(-1) == head_dim, "head_dim mismatch");
+    TORCH_CHECK(q.stride(-1) == 1, "q must have contiguous channels");
+    TORCH_CHECK(q.size(-2) > 0 && q.size(-2) % c.kv_heads == 0, "query_heads must be divisible by kv_heads");
+    const int64_t tokens = q.dim() == 4 ? q.size(1) : 1;
+    TORCH_CHECK(tokens > 0, "at least one token is required");
+    TORCH_CHECK(q.size(-2) <= 0x7fffffff && tokens <= 0x7fffffff, "q has a dimension beyond 32 bits");
+    const c10::cuda::CUDAGuard guard(pool.device());
+    mk36_kv4_attention_args a{};
+    torch::Tensor out = torch::empty(q.sizes(), q.options());
+    a.q = q.data_ptr();
+    a.out = out.data_ptr();
+    a.q_row = q.stride(0);
+    a.q_token = q.dim() == 4 ? q.stride(1) : 0;
+    a.q_head = q.stride(-2);
+    a.query_heads = static_cast<int32_t>(q.size(-2));
+    a.tokens = static_cast<int32_t>(tokens);
+    a.scale = static_cast<float>(scale);
+    const size_t bytes = mk36_kv4_attention_workspace_bytes(&c, &a);
+    TORCH_CHECK(bytes > 0, mk36_last_error());
+    torch::Tensor scratch = torch::empty({static_cast<int64_t>(bytes)}, pool.options());
+    check_rc(mk36_kv4_attention_decode(&c, &a, scratch.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
+// The three page operators: tables in, tables out (new ones, or the same with inplace) and the status on the device.
+using PageTables = std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>;
+
+PageTables kv_pages_call(const torch::Tensor& pages, const torch::Tensor& lengths, const torch::Tensor& refcounts, bool inplace, mk36_kv_pages_args a,
+                         int (*call)(const mk36_kv_pages_args*, void*, size_t, void*)) {
+    SHIM_CHECK_CUDA(pages);
+    check_int_table(pages, pages, "pages", 2);
+    check_int_table(lengths, pages, "lengths", 1);
+    check_int_table(refcounts, pages, "refcounts", 1);
+    TORCH_CHECK(lengths.size(0) == pages.size(0), "lengths must have an entry for each row of pages");
+    TORCH_CHECK(pages.size(0) <= 0x7fffffff && pages.size(1) <= 0x7fffffff, "pages has a dimension beyond 32 bits");
+    const c10::cuda::CUDAGuard guard(pages.device());
+    torch::Tensor new_pages = inplace ? pages : torch::empty_like(pages), new_lengths = inplace ? lengths : torch::empty_like(lengths);
+    torch::Tensor new_refs = inplace ? refcounts : torch::empty_like(refcounts), status = torch::empty({1}, pages.options());
+    a.page_table_in = pages.data_ptr<int32_t>();
+    a.lengths_in = lengths.data_ptr<int32_t>();
+    a.refcounts_in = refcounts.data_ptr<int32_t>();
+    a.page_table_out = new_pages.data_ptr<int32_t>();
+    a.lengths_out = new_lengths.data_ptr<int32_t>();
+    a.refcounts_out = new_refs.data_ptr<int32_t>();
+    a.status = status.data_ptr<int32_t>();
+    a.pages = refcounts.size(0);
+    a.rows = static_cast<int32_t>(pages.size(0));
+    a.row_pages = static_cast<int32_t>(pages.size(1));
+    const size_t bytes = mk36_kv_pages_workspace_bytes(&a);
+    torch::Tensor scratch = torch::empty({static_cast<int64_t>(bytes > 0 ? bytes : 4)}, pages.options().dtype(torch::kUInt8));
+    if (inplace)
+        for (const torch::Tensor* t : {&pages, &lengths, &refcounts}) t->unsafeGetTensorImpl()->bump_version();
+    check_rc(call(&a, scratch.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()));
+    return {new_pages, new_lengths, new_refs, status};
+}
+
+mk36_kv_pages_args kv_pages_pool(const torch::Tensor& pool, const torch::Tensor& pages, const torch::Tensor& refcounts) {
+    SHIM_CHECK_INPUT(pool);
+    TORCH_CHECK(pool.scalar_type() == torch::kUInt8 && pool.dim() == 4, "pool must be uint8 [pages, kv_heads, page_size / 16, tile_bytes]");
+    TORCH_CHECK(pages.device() == pool.device(), "pages must be on the device of the pool");
+    TORCH_CHECK(refcounts.dim() == 1 && refcounts.size(0) == pool.size(0), "refcounts must have an entry for each page of the pool");
+    TORCH_CHECK(pool.size(1) <= 0x7fffffff && pool.size(2) * 16 <= 0x7fffffff && pool.size(3) <= 0x7fffffff, "pool has a dimension beyond 32 bits");
+    mk36_kv_pages_args a{};
+    a.pool = pool.data_ptr();
+    a.kv_heads = static_cast<int32_t>(pool.size(1));
+    a.page_size = static_cast<int32_t>(pool.size(2) * 16);
+    a.tile_bytes = static_cast<int32_t>(pool.size(3));
+    return a;
+}
+
+PageTables kv_pages_fork(torch::Tensor pages, torch::Tensor lengths, torch::Tensor refcounts, torch::Tensor parents, torch::Tensor children, bool inplace) {
+    check_int_table(parents, pages, "parents", 1);
+    check_int_table(children, pages, "children", 1);
+    TORCH_CHECK(parents.size(0) == children.size(0), "parents and children must have one length");
+    TORCH_CHECK(parents.size(0) <= 0x7fffffff, "too many children");
+    mk36_kv_pages_args a{};
+    a.parents = parents.data_ptr<int32_t>();
+    a.children = children.data_ptr<int32_t>();
+    a.count = static_cast<int32_t>(parents.size(0));
+    return kv_pages_call(pages, lengths, refcounts, inplace, a, mk36_kv_pages_fork);
+}
+
+PageTables kv_pages_resize(torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, torch::Tensor refcounts, torch::Tensor new_lengths, bool inplace) {
+    mk36_kv_pages_args a = kv_pages_pool(pool, pages, refcounts);
+    check_int_table(new_lengths, pool, "new_lengths", 1);
+    TORCH_CHECK(new_lengths.size(0) == pages.size(0), "new_lengths must have an entry for each row of pages");
+    a.new_lengths = new_lengths.data_ptr<int32_t>();
+    pool.unsafeGetTensorImpl()->bump_version();
+    return kv_pages_call(pages, lengths, refcounts, inplace, a, mk36_kv_pages_resize);
+}
+
+PageTables kv_pages_compact(torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, torch::Tensor refcounts, bool inplace) {
+    mk36_kv_pages_args a = kv_pages_pool(pool, pages, refcounts);
+    pool.unsafeGetTensorImpl()->bump_version();
+    return kv_pages_call(pages, lengths, refcounts, inplace, a, mk36_kv_pages_compact);
+}
+
 // Reads back the device status word of this device's workspace (synchronises the stream).
 int64_t workspace_status(torch::Tensor like) {
     SHIM_CHECK_CUDA(like);
@@ -643,6 +833,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_attention_decode_steps", &linear_attention_decode_steps, "several recurrent steps in one launch, state resident on chip",
           py::arg("q"), py::arg("k"), py::arg("v"), py::arg("state"), py::arg("decay") = 1.0,
           py::arg("decay_per_step") = py::none(), py::arg("beta_per_step") = py::none(), py::arg("inplace") = false);
+    m.def("kv4_append", &kv4_append, "quantise tokens into the 4-bit paged cache", py::arg("pool"), py::arg("pages"), py::arg("lengths"),
+          py::arg("head_dim"), py::arg("k"), py::arg("v"), py::arg("cu_tokens") = py::none());
+    m.def("kv4_read", &kv4_read, "read tokens of the 4-bit paged cache into k and v", py::arg("pool"), py::arg("pages"), py::arg("lengths"),
+          py::arg("head_dim"), py::arg("k"), py::arg("v"), py::arg("cu_tokens") = py::none());
+    m.def("kv4_attention_decode", &kv4_attention_decode, "attention over the 4-bit paged cache (sm_100a)");
+    m.def("kv_pages_fork", &kv_pages_fork, "rows that share another row's pages");
+    m.def("kv_pages_resize", &kv_pages_resize, "take, free and copy pages for new lengths");
+    m.def("kv_pages_compact", &kv_pages_compact, "move the pages in use to the front of the pool");
     m.def("workspace_status", &workspace_status, "device status word of the workspace on the tensor's device");
     m.def("workspace_reset", &workspace_reset, "re-initialise the workspace on the tensor's device");
     m.def("library_version", []() { return mk36_version(); });

@@ -88,6 +88,39 @@ class LinearAttentionStepsArgs(C.Structure):
     ]
 
 
+class Kv4Cache(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p), ("page_table", C.c_void_p), ("lengths", C.c_void_p), ("pages", C.c_int64),
+        ("dtype", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+        ("rows", C.c_int32), ("row_pages", C.c_int32),
+    ]
+
+
+class Kv4Tokens(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("cu_tokens", C.c_void_p), ("tokens", C.c_int64),
+        ("k_row", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64),
+        ("v_row", C.c_int64), ("v_token", C.c_int64), ("v_head", C.c_int64),
+    ]
+
+
+class Kv4AttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("q_row", C.c_int64), ("q_token", C.c_int64), ("q_head", C.c_int64),
+        ("query_heads", C.c_int32), ("tokens", C.c_int32), ("scale", C.c_float),
+    ]
+
+
+class KvPagesArgs(C.Structure):
+    _fields_ = [
+        ("page_table_in", C.c_void_p), ("lengths_in", C.c_void_p), ("refcounts_in", C.c_void_p),
+        ("page_table_out", C.c_void_p), ("lengths_out", C.c_void_p), ("refcounts_out", C.c_void_p), ("status", C.c_void_p),
+        ("pool", C.c_void_p), ("new_lengths", C.c_void_p), ("parents", C.c_void_p), ("children", C.c_void_p),
+        ("pages", C.c_int64), ("rows", C.c_int32), ("row_pages", C.c_int32), ("count", C.c_int32), ("kv_heads", C.c_int32),
+        ("page_size", C.c_int32), ("tile_bytes", C.c_int32),
+    ]
+
+
 MK36_MAX_RANKS = 8
 MK36_IPC_HANDLE_BYTES = 64
 
@@ -121,6 +154,14 @@ SIGNATURES = {
     "mk36_static_scratch_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
     "mk36_linear_attention_decode": (C.c_int, [C.POINTER(LinearAttentionArgs), C.c_void_p]),
     "mk36_linear_attention_decode_steps": (C.c_int, [C.POINTER(LinearAttentionStepsArgs), C.c_void_p]),
+    "mk36_kv4_append": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4Tokens), C.c_void_p]),
+    "mk36_kv4_read": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4Tokens), C.c_void_p]),
+    "mk36_kv4_attention_workspace_bytes": (C.c_size_t, [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs)]),
+    "mk36_kv4_attention_decode": (C.c_int, [C.POINTER(Kv4Cache), C.POINTER(Kv4AttentionArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mk36_kv_pages_workspace_bytes": (C.c_size_t, [C.POINTER(KvPagesArgs)]),
+    "mk36_kv_pages_fork": (C.c_int, [C.POINTER(KvPagesArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mk36_kv_pages_resize": (C.c_int, [C.POINTER(KvPagesArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mk36_kv_pages_compact": (C.c_int, [C.POINTER(KvPagesArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "mk36_comm_buffer_bytes": (C.c_size_t, []),
     "mk36_comm_buffer_alloc": (C.c_int, [C.POINTER(C.c_void_p)]),
     "mk36_comm_buffer_reset": (C.c_int, [C.c_void_p, C.c_void_p]),
