@@ -27,7 +27,6 @@ namespace mk36 {
 
 constexpr int kKaWarps = 4;
 constexpr int kKaThreads = kKaWarps * 32;
-constexpr int kKaCtasPerSm = 2;
 constexpr int kKaMinTiles = 8;     // fewest tiles of a piece: two a warp
 constexpr int kKaJoinThreads = 256;
 
@@ -42,23 +41,29 @@ struct Kv4AttnParams {
     int streams;                              // kv_heads * blocks: passes over a row
     int ctas, wide_q;
     float scale;
+    FastDiv fd_blocks, fd_group, fd_streams;
 };
 
 // Partial results: per (CTA, first or last segment) and column the sums, then maximum (of scores in units of log 2) and sum of weights.
 __host__ __device__ constexpr int ka_slot_floats(int d, int nt) { return 8 * nt * (d + 4); }
 
+// What their registers leave room for.
+__host__ __device__ constexpr int ka_ctas_per_sm(bool fp32, int nt) { return fp32 || nt == 2 ? 2 : 3; }
+
 template <typename T, int D, int NT>
 struct KaConfig {
     static constexpr int kGroups = D / kKv4Group;
     static constexpr int kTile = kv4_tile_bytes(D, sizeof(T));
-    static constexpr int kFoldRow = D + 4;  // lanes 8 j + g of a store fall into 32 banks
-    static constexpr int kFold = kKaWarps * 8 * kFoldRow * 4;
-    static constexpr int kStats = kKaWarps * 8 * NT * (2 + kGroups) * 4;
-    static constexpr int kRoom = 232448 / kKaCtasPerSm - 1024 - kFold - kStats - 512;
+    static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kCtas = ka_ctas_per_sm(sizeof(T) == 4, NT);
+    static constexpr int kFoldRow = D + 8;  // the lanes of a store (g, j), rows j apart, fall into 32 banks
+    static constexpr int kFold = kKaWarps * 4 * kFoldRow * 4;
+    static constexpr int kOperands = NT * kQParts * kGroups * 4 * 32 * 8;  // of the queries
+    static constexpr int kStats = (kKaWarps * 8 * NT * 2 + 8 * NT * kGroups * 2) * 4;
+    static constexpr int kRoom = 232448 / kCtas - 1024 - kFold - kOperands - kStats - 512;
     static constexpr int kMost = kRoom / (kKaWarps * kTile);
     static constexpr int kStages = kMost < 8 ? kMost : 8;
-    static constexpr int kSmem = kKaWarps * kStages * kTile + kFold + kStats + kKaWarps * kStages * 8;
-    static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kSmem = kKaWarps * kStages * kTile + kFold + kOperands + kStats + kKaWarps * kStages * 8;
     static_assert(kStages >= 2, "no room for a ring");
 };
 
@@ -76,6 +81,13 @@ __device__ __forceinline__ void transpose8(float& x, float& y) {
     y = __uint_as_float(__byte_perm(lo, hi, 0x7632));
 }
 
+// D += A B, 16 x 16 by 16 x 8; not volatile, so that the compiler may place it
+__device__ __forceinline__ void ka_mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -87,16 +99,25 @@ __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
     return *reinterpret_cast<const unsigned*>(&h);
 }
 
+// x - h, one instruction
+__device__ __forceinline__ float minus_half(float x, __half h) {
+    float d;
+    asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(d) : "h"(*reinterpret_cast<const unsigned short*>(&h)), "h"((unsigned short)0xbc00), "f"(x));
+    return d;
+}
+
 // hi and lo halves of two fp32 values: 22 bits together
 __device__ __forceinline__ void split_half(float x, float y, unsigned& hi, unsigned& lo) {
     const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
     hi = *reinterpret_cast<const unsigned*>(&h);
-    lo = pack_half(x - f.x, y - f.y);
+    lo = pack_half(minus_half(x, __low2half(h)), minus_half(y, __high2half(h)));
 }
 
 // 2^e, e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// 2^e <= most < 2^(e + 1), within what pow2 takes on either side
+__device__ __forceinline__ int ka_exponent(float most) { return min(max((int)(__float_as_uint(most) >> 23), 14), 254) - 127; }
 
 template <int N>
 __device__ __forceinline__ void lds_words(const unsigned char* p, unsigned (&w)[N]) {
@@ -153,8 +174,8 @@ __device__ __forceinline__ void ka_advance(const Kv4AttnParams& p, KaCursor& c, 
 
 // All CTAs cut the line alike: tiles of all rows, and the piece length.  Every thread calls it; s: 32 words.
 template <int kThreads>
-__device__ __forceinline__ long long ka_line(const Kv4AttnParams& p, int rows, int* s) {
-    int mine = 0;  // tiles of a pass over every row: below 2^31 as long as rows * capacity / 16 is, which the host checks
+__device__ __forceinline__ int ka_line(const Kv4AttnParams& p, int rows, int* s) {
+    int mine = 0;  // the whole line is below 2^31 tiles, which the host sees to
     for (int r = threadIdx.x; r < rows; r += kThreads) mine += ka_tiles(p.cache, r);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(kFullMask, mine, off);
@@ -164,16 +185,15 @@ __device__ __forceinline__ long long ka_line(const Kv4AttnParams& p, int rows, i
     int sum = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) sum += s[w];
-    return (long long)sum * p.streams;
+    return sum * p.streams;
 }
 
-__device__ __forceinline__ long long ka_piece(long long total, int ctas) {
-    const long long each = (total + ctas - 1) / ctas;
-    return each < kKaMinTiles ? kKaMinTiles : each;
+__device__ __forceinline__ int ka_piece(int total, int ctas) {
+    return max(kKaMinTiles, (int)(((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas));
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel(const __grid_constant__ Kv4AttnParams p) {
+__global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_attention_kernel(const __grid_constant__ Kv4AttnParams p) {
     using C = KaConfig<T, D, NT>;
     constexpr int G = C::kGroups, QP = C::kQParts;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -181,10 +201,12 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
     unsigned char* ring = smem + warp * C::kStages * C::kTile;
     float* s_fold = reinterpret_cast<float*>(smem + kKaWarps * C::kStages * C::kTile);
-    float* s_max = s_fold + C::kFold / 4;               // [warp][8 NT]
+    uint2* s_qf = reinterpret_cast<uint2*>(s_fold + C::kFold / 4);  // [NT][QP][G][4][32]: operand registers of the queries
+    float* s_max = reinterpret_cast<float*>(s_qf) + C::kOperands / 4;  // [warp][8 NT]
     float* s_sum = s_max + kKaWarps * 8 * NT;           // [warp][8 NT]
-    float* s_zero = s_sum + kKaWarps * 8 * NT;          // [warp][8 NT][G]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(s_zero + kKaWarps * 8 * NT * G) + warp * C::kStages;
+    float* s_most = s_sum + kKaWarps * 8 * NT;          // [G][8 NT]: largest |q|
+    float* s_qsum = s_most + G * 8 * NT;                // [8 NT][G]
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(s_qsum + 8 * NT * G) + warp * C::kStages;
     if (lane == 0) {
         for (int i = 0; i < C::kStages; ++i) mbar_init(&bars[i], 1);
         mbar_init_fence();
@@ -193,14 +215,14 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
     asm volatile("griddepcontrol.launch_dependents;");  // the join may be set up while this runs; it waits for the end of the grid
 
     // ---- this CTA's piece of the line
-    const long long total = ka_line<kKaThreads>(p, p.cache.rows, s_scan);
-    const long long piece = ka_piece(total, p.ctas);
-    const long long begin = blockIdx.x * piece, end = min(total, begin + piece);
-    if (begin >= end) return;
+    const int total = ka_line<kKaThreads>(p, p.cache.rows, s_scan);
+    const int piece = ka_piece(total, p.ctas);
+    if ((long long)blockIdx.x * piece >= total) return;
+    const int begin = blockIdx.x * piece, end = total - begin < piece ? total : begin + piece;
     {
         // the row that holds tile `begin`: rows in batches of a thread each
         int before = 0;
-        const int target = (int)(begin / p.streams);  // begin's row has before * streams <= begin < (before + tiles) * streams
+        const int target = fdiv(begin, p.fd_streams);  // begin's row has before * streams <= begin < (before + tiles) * streams
         for (int base = 0;; base += kKaThreads) {
             const int r = base + threadIdx.x;
             const int n = r < p.cache.rows ? ka_tiles(p.cache, r) : 0;
@@ -230,121 +252,136 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
     start.row = s_start[0];
     start.tiles = ka_tiles(p.cache, start.row);
     {
-        const int off = (int)(begin - (long long)s_start[1] * p.streams);
-        start.stream = off / start.tiles;
+        const int off = begin - s_start[1] * p.streams;
+        start.stream = (unsigned)off / (unsigned)start.tiles;
         start.tile = off - start.stream * start.tiles;
     }
 
-    // ---- the ring: this warp's tiles are begin + warp, begin + warp + kKaWarps, ...
-    KaCursor ahead = start;  // the tile to be requested next
-    long long ahead_at = begin + warp;
-    ka_advance(p, ahead, warp);
-    int ahead_page = 0;
-    auto page_of = [&]() {
-        return ahead_at < end ? p.cache.table[(long long)ahead.row * p.cache.row_pages + fdiv(ahead.tile, p.cache.tiles_per_page)] : 0;
+    // ---- the ring: this warp's tiles are begin + warp, begin + warp + kKaWarps, ...  Lane i looks up where the i-th of the next 32 lies,
+    // a batch ahead, so that no request waits for the table
+    KaCursor place = start;
+    int place_at = begin + warp + kKaWarps * lane;
+    if (place_at < end) ka_advance(p, place, warp + kKaWarps * lane);
+    auto look_up = [&]() -> const unsigned char* {
+        const unsigned char* src = nullptr;  // null: the table names no page of the pool
+        if (place_at < end) {
+            int slot, inner;
+            fdivmod(place.tile, p.cache.tiles_per_page, slot, inner);
+            const long long page = p.cache.table[(long long)place.row * p.cache.row_pages + slot];
+            if (page >= 0 && page < p.cache.pages)
+                src = p.cache.pool + ((page * p.cache.kv_heads + fdiv(place.stream, p.fd_blocks)) * (int)p.cache.tiles_per_page.d + inner) * C::kTile;
+            place_at += 32 * kKaWarps;
+            if (place_at < end) ka_advance(p, place, 32 * kKaWarps);
+        }
+        return src;
     };
-    ahead_page = page_of();
+    const unsigned char *src_now = look_up(), *src_next = nullptr;
     int requested = 0;
-    unsigned lost = 0;  // bit s: stage s holds another page's tile, because the table names none
+    unsigned lost = 0;  // bit s: stage s holds another tile, because the table names none
     auto request = [&](int stage) {
-        if (ahead_at >= end) return;
-        const bool bad = ahead_page < 0 || ahead_page >= p.cache.pages;
-        lost = (lost & ~(1u << stage)) | (bad ? 1u << stage : 0u);
+        if (begin + warp + requested * kKaWarps >= end) return;
+        if (requested % 32 == 0) {
+            if (requested > 0) src_now = src_next;
+            src_next = look_up();
+        }
+        const unsigned char* src = reinterpret_cast<const unsigned char*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(src_now), requested % 32));
+        lost = (lost & ~(1u << stage)) | (src ? 0u : 1u << stage);
         if (lane == 0) {
-            const int per = (int)p.cache.tiles_per_page.d;
-            const int inner = ahead.tile - fdiv(ahead.tile, p.cache.tiles_per_page) * per;
-            const long long page = bad ? 0 : ahead_page;
-            const unsigned char* src = p.cache.pool + ((page * p.cache.kv_heads + ahead.stream / p.blocks) * per + inner) * C::kTile;
             mbar_arrive_expect_tx(&bars[stage], C::kTile);
-            bulk_copy_g2s(ring + stage * C::kTile, src, C::kTile, &bars[stage]);
+            bulk_copy_g2s(ring + stage * C::kTile, src ? src : p.cache.pool, C::kTile, &bars[stage]);
         }
         ++requested;
-        ka_advance(p, ahead, kKaWarps);
-        ahead_at += kKaWarps;
-        ahead_page = page_of();
     };
     __syncwarp();
     for (int i = 0; i < C::kStages; ++i) request(i);
 
     int stage = 0, use = 0;
     bool dead = false;  // a wait has run out: outputs from here on are NaN
-    long long at = begin + warp, segment = begin;
+    int at = begin + warp, segment = begin;
     KaCursor now = start;  // the tile at `segment`
     while (segment < end) {
-        const long long segment_end = min(end, segment + (now.tiles - now.tile));
-        const bool whole = now.tile == 0 && segment + now.tiles == segment_end;
+        const int segment_end = end - segment < now.tiles - now.tile ? end : segment + (now.tiles - now.tile);
+        const bool whole = now.tile == 0 && segment_end - segment == now.tiles;
         const int length = kv4_length(p.cache, now.row);
-        const int kv_head = now.stream / p.blocks, block = now.stream - kv_head * p.blocks;
+        const int kv_head = fdiv(now.stream, p.fd_blocks), block = now.stream - kv_head * p.blocks;
         const int row = now.row;
 
-        // ---- the queries of this pass: column g of each n-tile, this lane's channels of every group
-        unsigned qf[NT][QP][G][4][2];
-        float q_sum[NT][2][G], mult[NT][2];
+        // ---- the queries of this pass.  A warp prepares one group of 64 channels of every column (lane: column g, channels 16 j .. + 15);
+        // the operand registers stay in shared memory, where every tile takes them from.
+        float q_sum[NT][2][G], mult[NT];  // sums of columns 2 j, 2 j + 1; factor of column g's scores, in units of log 2
         int limit[NT][2], own_limit[NT];  // positions that the columns 2 j, 2 j + 1 see, and column g
+        {
+            float q[NT][16];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int column = (block * NT + nt) * 8 + g;
-            float q[G][16], most = 0.f;
-            const int token = column / p.group, head = kv_head * p.group + column - token * p.group;
-            const T* src = static_cast<const T*>(p.q) + row * p.q_row + token * p.q_token + head * p.q_head + 16 * j;
+            for (int nt = 0; nt < NT; ++nt) {
+                const int column = (block * NT + nt) * 8 + g, token = fdiv(column, p.fd_group);
+                own_limit[nt] = length - p.tokens + 1 + token;
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
+                for (int i = 0; i < 16; ++i) q[nt][i] = 0.f;
+                if (warp >= G) continue;
+                float most = 0.f;
+                if (column < p.columns) {
+                    const T* src = static_cast<const T*>(p.q) + row * p.q_row + token * p.q_token + (kv_head * p.group + column - token * p.group) * p.q_head +
+                                   warp * kKv4Group + 16 * j;
+                    if (p.wide_q) {
+                        float f[2][8];
+                        unpack8(load_chunk8<T>(src), f[0]);
+                        unpack8(load_chunk8<T>(src + 8), f[1]);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (column < p.columns) {
-                        const T* x = src + gr * kKv4Group + half * 8;
-                        if (p.wide_q) {
-                            unpack8(load_chunk8<T>(x), f);
-                        } else {
+                        for (int i = 0; i < 16; ++i) q[nt][i] = f[i >> 3][i & 7];
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) f[i] = to_float<T>(x[i]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        q[gr][half * 8 + i] = f[i];
-                        most = fmaxf(most, fabsf(f[i]));
+                        for (int i = 0; i < 16; ++i) q[nt][i] = to_float<T>(src[i]);
                     }
                 }
-            }
-            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-            const int e = min(max((int)(__float_as_uint(most) >> 23), 14), 254) - 127;  // 2^e <= most < 2^(e + 1)
-            const float up = pow2(14 - e);
-            float sum[G];
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-                sum[gr] = 0.f;
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(q[nt][i]));
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+                if (j == 0) s_most[warp * 8 * NT + nt * 8 + g] = most;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (warp >= G) continue;
+                float most = 0.f;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) most = fmaxf(most, s_most[gr * 8 * NT + nt * 8 + g]);
+                const float up = copysignf(pow2(14 - ka_exponent(most)), p.scale);  // the scale's sign goes into q
+                float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    q[gr][i] *= up;
-                    sum[gr] += q[gr][i];
+                    q[nt][i] *= up;
+                    sum += q[nt][i];
                 }
-                sum[gr] += __shfl_xor_sync(kFullMask, sum[gr], 1);
-                sum[gr] += __shfl_xor_sync(kFullMask, sum[gr], 2);
+                sum += __shfl_xor_sync(kFullMask, sum, 1);
+                sum += __shfl_xor_sync(kFullMask, sum, 2);
+                if (j == 0) s_qsum[(nt * 8 + g) * G + warp] = sum * pow2(-24);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {  // MMA m takes the codes 2 (m % 2), + 1, + 4, + 5 of word m / 2
                     const int c = (m >> 1) * 8 + (m & 1) * 2;
-                    if (QP == 1) {
-                        qf[nt][0][gr][m][0] = pack_half(q[gr][c], q[gr][c + 4]);
-                        qf[nt][0][gr][m][1] = pack_half(q[gr][c + 1] * 0.0625f, q[gr][c + 5] * 0.0625f);
-                    } else {
-                        split_half(q[gr][c], q[gr][c + 4], qf[nt][0][gr][m][0], qf[nt][QP - 1][gr][m][0]);
-                        split_half(q[gr][c + 1] * 0.0625f, q[gr][c + 5] * 0.0625f, qf[nt][0][gr][m][1], qf[nt][QP - 1][gr][m][1]);
-                    }
+                    uint2 hi, lo;
+                    split_half(q[nt][c], q[nt][c + 4], hi.x, lo.x);
+                    split_half(q[nt][c + 1] * 0.0625f, q[nt][c + 5] * 0.0625f, hi.y, lo.y);
+                    s_qf[(((nt * QP) * G + warp) * 4 + m) * 32 + lane] = hi;
+                    if (QP == 2) s_qf[(((nt * QP + QP - 1) * G + warp) * 4 + m) * 32 + lane] = lo;
                 }
             }
-            own_limit[nt] = length - p.tokens + 1 + token;
-            // what belongs to a column goes to the lanes that hold it in the scores' layout: columns 2 j, 2 j + 1
+            __syncthreads();
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int from = (2 * j + c) * 4;
+            for (int nt = 0; nt < NT; ++nt) {
+                float most = 0.f;
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) q_sum[nt][c][gr] = __shfl_sync(kFullMask, sum[gr], from) * pow2(-24);
-                const int e_c = __shfl_sync(kFullMask, e, from);
-                mult[nt][c] = ldexpf(p.scale * 1.4426950408889634f, 24 - 14 + e_c);
-                limit[nt][c] = __shfl_sync(kFullMask, own_limit[nt], from);
+                for (int gr = 0; gr < G; ++gr) most = fmaxf(most, s_most[gr * 8 * NT + nt * 8 + g]);
+                // not 0, so that a score of -infinity stays one
+                mult[nt] = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, 24 - 14 + ka_exponent(most)), 1e-37f);
+                // what belongs to a column, for the lanes that hold it in the products' layout: columns 2 j, 2 j + 1
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) q_sum[nt][c][gr] = s_qsum[(nt * 8 + 2 * j + c) * G + gr];
+                    limit[nt][c] = __shfl_sync(kFullMask, own_limit[nt], (2 * j + c) * 4);
+                }
             }
         }
         int sees_all = length;  // every column sees the positions below this
@@ -367,10 +404,11 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
                     for (int i = 0; i < 4; ++i) o[nt][gr][m][i] = 0.f;
             }
         }
-        int unit = 1;  // exponent field of the power of two that weights times scales are divided by
+        int unit = 1, unit_limit = 0;  // exponent field of the power of two that weights times scales are divided by; none yet
+        float shrink = pow2(126);
 
         for (; at < segment_end; at += kKaWarps) {
-            const int tile = now.tile + (int)(at - segment);
+            const int tile = now.tile + (at - segment);
             if (!dead && !mbar_wait(&bars[stage], use & 1, &s_abort)) dead = true;
             dead = __any_sync(kFullMask, dead);
             if (dead || (lost >> stage & 1u)) {
@@ -392,36 +430,42 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
                 load_params<T, G>(params + g * (G * 2 * (int)sizeof(T)), ks[0], kz[0]);
                 load_params<T, G>(params + (g + 8) * (G * 2 * (int)sizeof(T)), ks[1], kz[1]);
                 constexpr int kUnit = D >= 128 ? 16 : 8, kVecs = D / 8 / kUnit, kWords = kUnit / 4;
+                unsigned a[kVecs][kWords], a8[kVecs][kWords];  // tokens g and g + 8
 #pragma unroll
                 for (int v = 0; v < kVecs; ++v) {
-                    unsigned a[kWords], b[kWords];
-                    lds_words(codes + (v * 32 + lane) * kUnit, a);
-                    lds_words(codes + ((kVecs + v) * 32 + lane) * kUnit, b);
+                    lds_words(codes + (v * 32 + lane) * kUnit, a[v]);
+                    lds_words(codes + ((kVecs + v) * 32 + lane) * kUnit, a8[v]);
+                }
+                float acc[NT][G][4];
 #pragma unroll
-                    for (int x = 0; x < kWords / 2; ++x) {
-                        const int gr = v * (kWords / 2) + x;
-                        float acc[NT][4];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
+                    for (int gr = 0; gr < G; ++gr)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
+                        for (int i = 0; i < 4; ++i) acc[nt][gr][i] = 0.f;
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            const unsigned wa = a[2 * x + (m >> 1)] >> (8 * (m & 1)), wb = b[2 * x + (m >> 1)] >> (8 * (m & 1));
-                            const unsigned a0 = wa & 0x000f000fu, a1 = wb & 0x000f000fu, a2 = wa & 0x00f000f0u, a3 = wb & 0x00f000f0u;
+                for (int m = 0; m < 4; ++m) {  // the groups' chains side by side: an MMA does not wait for the one before it
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
+                    for (int gr = 0; gr < G; ++gr) {
+                        const int v = gr / (kWords / 2), x = 2 * (gr % (kWords / 2)) + (m >> 1);
+                        const unsigned wa = a[v][x] >> (8 * (m & 1)), wb = a8[v][x] >> (8 * (m & 1));
+                        const unsigned a0 = wa & 0x000f000fu, a1 = wb & 0x000f000fu, a2 = wa & 0x00f000f0u, a3 = wb & 0x00f000f0u;
 #pragma unroll
-                                for (int part = 0; part < QP; ++part)
-                                    mma_16816<__half>(acc[nt], a0, a1, a2, a3, qf[nt][part][gr][m][0], qf[nt][part][gr][m][1]);
-                        }
+                        for (int part = 0; part < QP; ++part)
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                s[nt][i] += fmaf(ks[i >> 1][gr], acc[nt][i], kz[i >> 1][gr] * q_sum[nt][i & 1][gr]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const uint2 b = s_qf[(((nt * QP + part) * G + gr) * 4 + m) * 32 + lane];
+                                ka_mma(acc[nt][gr], a0, a1, a2, a3, b.x, b.y);
+                            }
                     }
                 }
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[nt][i] = fmaf(ks[i >> 1][gr], acc[nt][gr][i], fmaf(kz[i >> 1][gr], q_sum[nt][i & 1][gr], s[nt][i]));
             }
             const int first = tile * kKv4Tile;
             const bool edge = first + kKv4Tile > sees_all;
@@ -429,7 +473,6 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[nt][i] *= mult[nt][i & 1];
                     if (edge && first + g + 8 * (i >> 1) >= limit[nt][i & 1]) s[nt][i] = -INFINITY;
                 }
                 // from (tokens g, g + 8; columns 2 j, 2 j + 1) to (tokens 2 j, 2 j + 1, + 8, + 9; column g)
@@ -448,18 +491,18 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
                     for (int gr = 0; gr < G; ++gr) vs[i][gr] = vz[i][gr] = 0.f;
                 }
             }
-            unsigned largest = 0;
+            // Weights times scales are divided by 2^(unit - 127): they stay below 2^15 as long as no scale's exponent passes unit + 13.
+            // The exponents' bits or'ed together are no smaller than the largest; only where that says so, it is looked for.
+            unsigned bits = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) largest = max(largest, __float_as_uint(vs[i][gr]));
-            largest = max(largest, __shfl_xor_sync(kFullMask, largest, 1));
-            largest = max(largest, __shfl_xor_sync(kFullMask, largest, 2));
-            const int unit_now = max(unit, min((int)(largest >> 23), 253));
+                for (int gr = 0; gr < G; ++gr) bits |= __float_as_uint(vs[i][gr]);
+            const bool larger = (int)(bits >> 23) > unit_limit;
 
             // ---- running maximum; what has been summed is brought to it
             float corr[NT];
-            bool moved = unit_now != unit;
+            bool moved = larger;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float m = fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3]));
@@ -467,13 +510,31 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
                 m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 2));
                 m = fmaxf(m, top[nt]);
                 const float base = m == -INFINITY ? 0.f : m;
-                corr[nt] = exp2_approx(top[nt] - base);
+                corr[nt] = exp2_approx((top[nt] - base) * mult[nt]);
                 moved |= m != top[nt];
                 top[nt] = m;
+                const float shift = base * mult[nt];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] = sizeof(T) == 4 ? exp2f(s[nt][i] - base) : exp2_approx(s[nt][i] - base);
+                for (int i = 0; i < 4; ++i) {
+                    // fp32: the difference first, which is exact where it matters
+                    s[nt][i] = sizeof(T) == 4 ? exp2f((s[nt][i] - base) * mult[nt]) : exp2_approx(fmaf(s[nt][i], mult[nt], -shift));
+                }
             }
             if (__any_sync(kFullMask, moved)) {
+                int unit_now = unit;
+                if (__any_sync(kFullMask, larger)) {
+                    unsigned largest = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) {
+                            const unsigned x = __float_as_uint(vs[i][gr]);
+                            largest = max(largest, x < 0x7f800000u ? x : 0u);  // a NaN is no size: other columns may not see it
+                        }
+                    largest = max(largest, __shfl_xor_sync(kFullMask, largest, 1));
+                    largest = max(largest, __shfl_xor_sync(kFullMask, largest, 2));
+                    unit_now = max(unit, min((int)(largest >> 23), 253));
+                }
                 const float down = pow2(max(unit - unit_now, -126));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -490,8 +551,9 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
                     }
                 }
                 unit = unit_now;
+                unit_limit = unit + 13;
+                shrink = pow2(127 - unit);
             }
-            const float shrink = pow2(127 - unit);
 
             // ---- values
             constexpr int kUnit = D / 16;
@@ -505,10 +567,8 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
                 auto weigh = [&](const float (&scale)[4][G], const float (&zero)[4][G]) {
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
-                        float add = s[nt][0] * zero[0][gr];
 #pragma unroll
-                        for (int i = 1; i < 4; ++i) add = fmaf(s[nt][i], zero[i][gr], add);
-                        zero_sum[nt][gr] += add;
+                        for (int i = 0; i < 4; ++i) zero_sum[nt][gr] = fmaf(s[nt][i], zero[i][gr], zero_sum[nt][gr]);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[nt][i] *= shrink;
@@ -533,23 +593,42 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
             }
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
+                unsigned a[4][4];
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {  // rows g and g + 8: channels 8 g + c and 8 g + c + 2, c = 0, 1 (x 16), 4, 5 (x 16)
                     const unsigned pick = m < 2 ? 0x5410u : 0x7632u, mask = m & 1 ? 0x00f000f0u : 0x000f000fu;
                     const unsigned near = __byte_perm(v[0][gr], v[1][gr], pick), far = __byte_perm(v[2][gr], v[3][gr], pick);
-                    const unsigned a0 = near & mask, a1 = near >> 8 & mask, a2 = far & mask, a3 = far >> 8 & mask;
+                    a[m][0] = near & mask, a[m][1] = near >> 8 & mask, a[m][2] = far & mask, a[m][3] = far >> 8 & mask;
+                }
+                if (sizeof(T) == 4) {  // chains of two, added up in fp32: the tensor core cuts off where an addition rounds
+                    float acc[NT][4][4];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if (sizeof(T) == 4) {  // chains of two, added up in fp32: the tensor core cuts off where an addition rounds
-                            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_16816<__half>(acc, a0, a1, a2, a3, lo[nt][gr][0], lo[nt][gr][1]);
-                            mma_16816<__half>(acc, a0, a1, a2, a3, hi[nt][gr][0], hi[nt][gr][1]);
-                            add_tile(o[nt][gr][m], acc);
-                        } else {
-                            mma_16816<__half>(o[nt][gr][m], a0, a1, a2, a3, lo[nt][gr][0], lo[nt][gr][1]);
-                            mma_16816<__half>(o[nt][gr][m], a0, a1, a2, a3, hi[nt][gr][0], hi[nt][gr][1]);
-                        }
-                    }
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[nt][m][i] = 0.f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) ka_mma(acc[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][gr][0], lo[nt][gr][1]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) ka_mma(acc[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][gr][0], hi[nt][gr][1]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) add_tile(o[nt][gr][m], acc[nt][m]);
+                } else {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) ka_mma(o[nt][gr][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][gr][0], lo[nt][gr][1]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) ka_mma(o[nt][gr][m], a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][gr][0], hi[nt][gr][1]);
                 }
             }
 
@@ -570,63 +649,61 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
             }
             if (j == 0) {
                 const int c = (warp * NT + nt) * 8 + g;
-                s_max[c] = top[nt];
+                s_max[c] = top[nt] * mult[nt];
                 s_sum[c] = weight_sum[nt];
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) s_zero[c * G + gr] = zero_sum[nt][gr];
             }
         }
         __syncthreads();
         const float grow = pow2(unit - 127);
+        const long long slot = 2ll * blockIdx.x + (segment > begin ? 1 : 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float weight[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < 2; ++c) {  // the columns 2 j + c of all warps; a warp then adds one of them up
                 float m = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kKaWarps; ++w) m = fmaxf(m, s_max[(w * NT + nt) * 8 + 2 * j + c]);
                 const float own = s_max[(warp * NT + nt) * 8 + 2 * j + c];
-                weight[c] = own == -INFINITY ? 0.f : exp2f(own - m) * grow;
-            }
-            // channel 8 g + i of a group at 8 i + g: the 32 lanes of a store fall into 32 banks
+                const float weight = own == -INFINITY ? 0.f : exp2f(own - m);
+                // channel 8 g + i of a group at 8 i + g
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr)
+                for (int gr = 0; gr < G; ++gr) {
+                    const float zero = __shfl_sync(kFullMask, zero_sum[nt][gr], (2 * j + c) * 4);
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int c = i & 1, channel = (m >> 1) * 4 + (m & 1) + 2 * (i >> 1);
-                        s_fold[(warp * 8 + 2 * j + c) * C::kFoldRow + gr * kKv4Group + channel * 8 + g] = o[nt][gr][m][i] * (m & 1 ? 0x1p20f : 0x1p24f) * weight[c];
+                    for (int k = 0; k < 8; ++k) {
+                        const int m4 = (k >> 2) * 2 + (k & 1), half = (k >> 1) & 1;  // channel 8 g + k lies in these registers
+                        const float sum = fmaf(o[nt][gr][m4][2 * half + c] * (m4 & 1 ? 0x1p20f : 0x1p24f), grow, zero);
+                        s_fold[(warp * 4 + j) * C::kFoldRow + gr * kKv4Group + k * 8 + g] = sum * weight;
                     }
-            __syncthreads();
-            const long long slot = 2ll * blockIdx.x + (segment > begin ? 1 : 0);
-            float* part = p.partial + slot * ka_slot_floats(D, NT) + nt * 8 * (D + 4);
-            for (int i = threadIdx.x; i < 8 * D; i += kKaThreads) {
-                const int c = i / D, channel = i - c * D;
-                const int column = (block * NT + nt) * 8 + c;
-                if (column >= p.columns) break;  // columns ascend with i
-                const int place = channel / kKv4Group * kKv4Group + channel % 8 * 8 + channel % kKv4Group / 8;
-                float m = -INFINITY, sum = 0.f, value = 0.f;
-#pragma unroll
-                for (int w = 0; w < kKaWarps; ++w) m = fmaxf(m, s_max[(w * NT + nt) * 8 + c]);
-#pragma unroll
-                for (int w = 0; w < kKaWarps; ++w) {
-                    const int x = (w * NT + nt) * 8 + c;
-                    const float own = s_max[x] == -INFINITY ? (s_sum[x] == 0.f ? 0.f : s_sum[x]) : exp2f(s_max[x] - m);
-                    sum = fmaf(own, s_sum[x], sum);
-                    value += s_fold[(w * 8 + c) * C::kFoldRow + place] + own * s_zero[x * G + channel / kKv4Group];
                 }
-                if (whole) {
-                    const int token = column / p.group, head = kv_head * p.group + column - token * p.group;
+                __syncthreads();
+                const int mine = 2 * warp + c, column = (block * NT + nt) * 8 + mine;
+                if (column < p.columns) {
+                    float most = -INFINITY, sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kKaWarps; ++w) most = fmaxf(most, s_max[(w * NT + nt) * 8 + mine]);
+#pragma unroll
+                    for (int w = 0; w < kKaWarps; ++w) {
+                        const int x = (w * NT + nt) * 8 + mine;
+                        sum += s_max[x] == -INFINITY ? s_sum[x] : exp2f(s_max[x] - most) * s_sum[x];  // without a maximum the sum is 0 or NaN
+                    }
+                    const int token = fdiv(column, p.fd_group), head = kv_head * p.group + column - token * p.group;
                     T* out = static_cast<T*>(p.out) + (((long long)row * p.tokens + token) * p.query_heads + head) * D;
-                    out[channel] = from_float<T>(sum == 0.f ? 0.f : value / sum);
-                } else {
-                    part[c * (D + 4) + channel] = value;
-                    if (channel < 2) part[c * (D + 4) + D + channel] = channel ? sum : m;
+                    float* part = p.partial + slot * ka_slot_floats(D, NT) + (nt * 8 + mine) * (D + 4);
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const int channel = i * 32 + lane, at = channel / kKv4Group * kKv4Group + channel % 8 * 8 + channel % kKv4Group / 8;
+                        float value = 0.f;
+#pragma unroll
+                        for (int w = 0; w < kKaWarps; ++w) value += s_fold[(w * 4 + warp) * C::kFoldRow + at];
+                        if (whole) out[channel] = from_float<T>(sum == 0.f ? 0.f : value * inv);
+                        else part[channel] = value;
+                    }
+                    if (!whole && lane < 2) part[D + lane] = lane ? sum : most;
                 }
+                __syncthreads();
             }
-            __syncthreads();
         }
         now.tile = now.tiles - 1;
         ka_advance(p, now, 1);
@@ -642,61 +719,79 @@ __global__ void __launch_bounds__(kKaThreads, kKaCtasPerSm) kv4_attention_kernel
     }
 }
 
-// Joins the partial results of rows that several CTAs worked on; a CTA for each query head and token.  Rows without a token get zeros.
+// Joins the partial results of rows that several CTAs worked on; a CTA for each query head, token and 64 channels.  Rows without a token
+// get zeros.  A warp takes every eighth partial result, kBatch of them in flight together, with a running maximum of its own.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kKaJoinThreads) kv4_attention_join_kernel(const __grid_constant__ Kv4AttnParams p) {
-    __shared__ float s_out[kKaJoinThreads / 32][D];
-    __shared__ int s_scan[kKaJoinThreads / 32];
+    constexpr int kWarps = kKaJoinThreads / 32, kBatch = 5;
+    __shared__ float2 s_out[kWarps][32];
+    __shared__ float s_max[kWarps], s_sum[kWarps];
+    __shared__ int s_scan[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.x % p.query_heads, rest = blockIdx.x / p.query_heads;
+    const int part = blockIdx.x % (D / 64), output = blockIdx.x / (D / 64);
+    const int head = output % p.query_heads, rest = output / p.query_heads;
     const int token = rest % p.tokens, row = rest / p.tokens;
     const int tiles = ka_tiles(p.cache, row);
-    T* out = static_cast<T*>(p.out) + (long long)blockIdx.x * D;
+    T* out = static_cast<T*>(p.out) + (long long)output * D + part * 64;
     if (tiles == 0) {
         asm volatile("griddepcontrol.wait;" ::: "memory");  // no CTA of this grid ends before the grid ahead of it
-        for (int c = threadIdx.x; c < D; c += kKaJoinThreads) out[c] = from_float<T>(0.f);
+        if (threadIdx.x < 64) out[threadIdx.x] = from_float<T>(0.f);
         return;
     }
-    const int kv_head = head / p.group, column = token * p.group + head - kv_head * p.group;
+    const int kv_head = fdiv(head, p.fd_group), column = token * p.group + head - kv_head * p.group;
     const int block = column / (8 * NT);
-    const long long before = ka_line<kKaJoinThreads>(p, row, s_scan), total = ka_line<kKaJoinThreads>(p, p.cache.rows, s_scan);
-    const long long piece = ka_piece(total, p.ctas);
-    const long long first = before + (long long)(kv_head * p.blocks + block) * tiles;
-    const long long cta0 = first / piece, cta1 = (first + tiles - 1) / piece;
+    const int before = ka_line<kKaJoinThreads>(p, row, s_scan), total = ka_line<kKaJoinThreads>(p, p.cache.rows, s_scan);
+    const int piece = ka_piece(total, p.ctas);
+    const int first = before + (kv_head * p.blocks + block) * tiles;
+    const int cta0 = (unsigned)first / (unsigned)piece, cta1 = (unsigned)(first + tiles - 1) / (unsigned)piece;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (cta0 == cta1) return;  // that CTA has written the output
     const float* base = p.partial + (column - block * 8 * NT) * (D + 4);
-    auto part_of = [&](long long cta) { return base + (2 * cta + (first > cta * piece ? 1 : 0)) * ka_slot_floats(D, NT); };
-    float top = -INFINITY;
-    for (long long c = cta0 + lane; c <= cta1; c += 32) top = fmaxf(top, __ldcg(part_of(c) + D));
-    top = warp_max(top);
-    constexpr int kPer = D / 32;
-    float acc[kPer], sum = 0.f;
+    float top = -INFINITY, sum = 0.f;
+    float2 acc = make_float2(0.f, 0.f);
+    for (int c0 = cta0 + warp; c0 <= cta1; c0 += kWarps * kBatch) {
+        float2 stats[kBatch], value[kBatch];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (long long c = cta0 + warp; c <= cta1; c += kKaJoinThreads / 32) {
-        const float* x = part_of(c);
-        const float m = __ldcg(x + D), part_sum = __ldcg(x + D + 1);
-        const float own = m == -INFINITY ? (part_sum == 0.f ? 0.f : part_sum) : exp2f(m - top);
-        sum = fmaf(own, part_sum, sum);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) acc[i] = fmaf(own, __ldcg(x + i * 32 + lane), acc[i]);
-    }
-    __shared__ float s_sum[kKaJoinThreads / 32];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) s_out[warp][i * 32 + lane] = acc[i];
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    for (int c = threadIdx.x; c < D; c += kKaJoinThreads) {
-        float value = 0.f, all = 0.f;
-#pragma unroll
-        for (int w = 0; w < kKaJoinThreads / 32; ++w) {
-            value += s_out[w][c];
-            all += s_sum[w];
+        for (int i = 0; i < kBatch; ++i) {
+            const int c = c0 + i * kWarps;
+            stats[i] = make_float2(-INFINITY, 0.f);
+            value[i] = make_float2(0.f, 0.f);
+            if (c <= cta1) {
+                const float* x = base + (2ll * c + (first > c * piece ? 1 : 0)) * ka_slot_floats(D, NT);
+                stats[i] = __ldcg(reinterpret_cast<const float2*>(x + D));
+                value[i] = __ldcg(reinterpret_cast<const float2*>(x + part * 64) + lane);
+            }
         }
-        out[c] = from_float<T>(all == 0.f ? 0.f : value / all);
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) now = fmaxf(now, stats[i].x);
+        const float base_now = now == -INFINITY ? 0.f : now, corr = exp2f(top - base_now);
+        sum *= corr, acc.x *= corr, acc.y *= corr;
+        top = now;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const float own = exp2f(stats[i].x - base_now);
+            sum += stats[i].x == -INFINITY ? stats[i].y : own * stats[i].y;  // without a maximum the sum is 0 or NaN
+            acc.x = fmaf(own, value[i].x, acc.x), acc.y = fmaf(own, value[i].y, acc.y);
+        }
     }
+    s_out[warp][lane] = acc;
+    if (lane == 0) s_max[warp] = top, s_sum[warp] = sum;
+    __syncthreads();
+    if (warp != 0) return;
+    float all_top = -INFINITY, all = 0.f;
+    float2 value = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all_top = fmaxf(all_top, s_max[w]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const float own = s_max[w] == -INFINITY ? 0.f : exp2f(s_max[w] - all_top);
+        all += s_max[w] == -INFINITY ? s_sum[w] : own * s_sum[w];
+        value.x = fmaf(own, s_out[w][lane].x, value.x), value.y = fmaf(own, s_out[w][lane].y, value.y);
+    }
+    const float inv = all == 0.f ? 0.f : 1.f / all;
+    out[2 * lane] = from_float<T>(all == 0.f ? 0.f : value.x * inv);
+    out[2 * lane + 1] = from_float<T>(all == 0.f ? 0.f : value.y * inv);
 }
 
 static int kv4_attention_params(const mk36_kv4_cache* c, const mk36_kv4_attention_args* a, Kv4AttnParams* p) {
@@ -708,10 +803,8 @@ static int kv4_attention_params(const mk36_kv4_cache* c, const mk36_kv4_attentio
     if (a->query_heads <= 0 || a->tokens <= 0) MK36_FAIL(MK36_ERR_INVALID_ARG, "%s: sizes must be positive", what);
     if (a->query_heads % c->kv_heads != 0) MK36_FAIL(MK36_ERR_INVALID_ARG, "%s: query_heads must be divisible by kv_heads", what);
     if (!(a->scale - a->scale == 0.0f)) MK36_FAIL(MK36_ERR_INVALID_ARG, "%s: scale must be finite", what);
-    if ((long long)c->rows * a->tokens > 0x7fffffffLL || (long long)c->rows * a->tokens * a->query_heads > 0x7fffffffLL)
-        MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 query heads", what);
-    if ((long long)c->rows * c->row_pages * (c->page_size / kKv4Tile) > 0x7fffffffLL)
-        MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: the table holds more than 2^31 - 1 tiles of 16 tokens", what);
+    if ((long long)c->rows * a->tokens > 0x7fffffffLL || (long long)c->rows * a->tokens * a->query_heads > 0x1fffffffLL)
+        MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: more than 2^29 - 1 query heads", what);
     const int elem = kv4_elem(c->dtype);
     if (reinterpret_cast<uintptr_t>(a->q) % elem != 0 || reinterpret_cast<uintptr_t>(a->out) % elem != 0)
         MK36_FAIL(MK36_ERR_INVALID_ARG, "%s: q and out must be aligned to their elements", what);
@@ -737,8 +830,11 @@ static int ka_grid(Kv4AttnParams* p, int dtype, int page_size) {
     const int nt = ka_blocks_of_eight(*p, dtype);
     p->blocks = (p->columns + 8 * nt - 1) / (8 * nt);
     p->streams = p->cache.kv_heads * p->blocks;
-    const long long most = (long long)p->cache.rows * p->cache.row_pages * (page_size / kKv4Tile) * p->streams;
-    const long long ctas = (most + kKaMinTiles - 1) / kKaMinTiles, resident = (long long)info->sm_count * kKaCtasPerSm;
+    p->fd_blocks = make_fastdiv((unsigned)p->blocks), p->fd_group = make_fastdiv((unsigned)p->group), p->fd_streams = make_fastdiv((unsigned)p->streams);
+    const double line = (double)p->cache.rows * p->cache.row_pages * (page_size / kKv4Tile) * p->streams;
+    if (line > 2e9) MK36_FAIL(MK36_ERR_UNSUPPORTED, "kv4_attention_decode: the table holds more than 2e9 tiles of 16 tokens, heads and query blocks");
+    const long long most = (long long)line;
+    const long long ctas = (most + kKaMinTiles - 1) / kKaMinTiles, resident = (long long)info->sm_count * ka_ctas_per_sm(dtype == MK36_F32, nt);
     p->ctas = (int)(ctas < resident ? ctas : resident);
     return MK36_OK;
 }
@@ -751,7 +847,7 @@ static int kv4_attention_launch(const Kv4AttnParams& p, cudaStream_t s) {
     kv4_attention_kernel<T, D, NT><<<p.ctas, kKaThreads, C::kSmem, s>>>(p);
     MK36_CUDA_OK(cudaGetLastError());
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)((long long)p.cache.rows * p.tokens * p.query_heads));
+    config.gridDim = dim3((unsigned)((long long)p.cache.rows * p.tokens * p.query_heads * (D / 64)));
     config.blockDim = dim3(kKaJoinThreads);
     config.stream = s;
     cudaLaunchAttribute early{};

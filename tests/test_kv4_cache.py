@@ -410,6 +410,24 @@ def test_a_nan_reaches_the_queries_that_see_it_and_no_other(cuda_device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq", [1, 4])
+def test_a_nan_does_not_reach_earlier_queries_of_a_draft(cuda_device, dtype, hq):
+    s = Server(cuda_device, dtype, 64, 1, 16, [70, 37])
+    k, v = s.tokens(107, seed=1)
+    k[69, 0, 5], v[70 + 35, 0, 9] = math.nan, math.inf  # the last token of row 0, the last but one of row 1
+    oracle.append(s.pool, s.table, s.lengths, k, v, s.lengths)
+    s.cache.pool.copy_(torch.from_numpy(s.pool))
+    q = torch.randn(2, 4, hq, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    out = mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu)
+    assert torch.isnan(out[0, 3]).all() and torch.isnan(out[1, 2:]).all()
+    early = mk.kv4_attention_decode(q[:, :2].contiguous().to(cuda_device), s.cache, mk.PageTable(s.gpu.pages, s.gpu.lengths - 2, s.gpu.refcounts))
+    s.lengths = [68, 35]
+    check_attention(s, q[:, :2], early)
+    check_attention(s, q[:, :2], out[:, :2])
+
+
+@pytest.mark.gpu
 def test_attention_takes_strided_and_unaligned_queries_and_a_negative_scale(cuda_device):
     s = Server(cuda_device, torch.float16, 128, 2, 16, [45, 3, 99])
     s.fill()
