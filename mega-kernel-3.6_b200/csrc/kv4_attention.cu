@@ -19,6 +19,8 @@
 // joins those.
 #include <math.h>
 
+#include <type_traits>
+
 #include "mk36_kv4.cuh"
 #include "mk36_mma.cuh"
 #include "mk36_ring.cuh"
@@ -113,6 +115,51 @@ __device__ __forceinline__ void split_half(float x, float y, unsigned& hi, unsig
     lo = pack_half(minus_half(x, __low2half(h)), minus_half(y, __high2half(h)));
 }
 
+// The two-byte types' parameters are worked on as they lie: pairs of halves in a word.
+template <typename T>
+struct KaPair;
+template <>
+struct KaPair<__nv_bfloat16> {
+    static constexpr unsigned kExponent = 0x7f80u, kTop = 255u;
+    static constexpr int kShift = 7, kLeast = 23, kBias = 127;
+    // scales as f16, 2^(unit - bias) as 2^7: a shift of the exponents.  Scales 2^21 times smaller than that become 0.
+    static __device__ __forceinline__ unsigned scales(unsigned w, int unit) {
+        const unsigned c = (unsigned)(unit - 22) * 0x00800080u;
+        return __vmaxu2(w, c) * 8u - c * 8u;
+    }
+    static __device__ __forceinline__ unsigned pack(float x, float y) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const unsigned*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(unsigned w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+};
+template <>
+struct KaPair<__half> {
+    static constexpr unsigned kExponent = 0x7c00u, kTop = 31u;
+    static constexpr int kShift = 10, kLeast = 7, kBias = 15;
+    static __device__ __forceinline__ unsigned scales(unsigned w, int unit) {
+        const unsigned f = (unsigned)(22 - unit + 15) * 0x04000400u;  // 2^(22 - unit), twice
+        const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&f));
+        return *reinterpret_cast<const unsigned*>(&h);
+    }
+    static __device__ __forceinline__ unsigned pack(float x, float y) { return pack_half(x, y); }
+    static __device__ __forceinline__ float2 unpack(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+};
+
+template <typename T>
+__device__ __forceinline__ void ka_mma_params(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    if (std::is_same<T, __nv_bfloat16>::value) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    } else {
+        ka_mma(d, a0, a1, a2, a3, b0, b1);
+    }
+}
+
+__device__ __forceinline__ __half2 as_half2(unsigned w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ unsigned as_word(__half2 h) { return *reinterpret_cast<const unsigned*>(&h); }
+
 // 2^e, e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
@@ -133,6 +180,28 @@ __device__ __forceinline__ void lds_words(const unsigned char* p, unsigned (&w)[
             w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
         }
     }
+}
+
+// Which halves of a pair of tokens t, t + 1 lie below `end`.
+__device__ __forceinline__ unsigned ka_keep(int t, int end) { return (t < end ? 0x0000ffffu : 0u) | (t + 1 < end ? 0xffff0000u : 0u); }
+
+// Weights (two halves) times scales, again in two halves: the product rounded, and what the rounding left plus the weights' second halves.
+__device__ __forceinline__ void ka_weigh(unsigned ph, unsigned pl, unsigned scale, unsigned& hi, unsigned& lo) {
+    const __half2 h = __hmul2(as_half2(ph), as_half2(scale));
+    hi = as_word(h);
+    lo = as_word(__hfma2(as_half2(pl), as_half2(scale), __hfma2(as_half2(ph), as_half2(scale), __hneg2(h))));
+}
+
+// The least unit, and what a sum in units of it is multiplied by.
+template <typename T>
+__device__ __forceinline__ int ka_least_unit() {
+    if constexpr (sizeof(T) == 4) return 1;
+    else return KaPair<T>::kLeast;
+}
+template <typename T>
+__device__ __forceinline__ float ka_unit_value(int unit) {
+    if constexpr (sizeof(T) == 4) return pow2(unit - 127);
+    else return pow2(unit - KaPair<T>::kBias - 7);
 }
 
 // Scales and zero points of a token's groups.
@@ -196,12 +265,13 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_attention_kernel(const __grid_constant__ Kv4AttnParams p) {
     using C = KaConfig<T, D, NT>;
     constexpr int G = C::kGroups, QP = C::kQParts;
+    constexpr bool kWide = sizeof(T) == 4;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int s_scan[kKaWarps], s_start[2], s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
     unsigned char* ring = smem + warp * C::kStages * C::kTile;
     float* s_fold = reinterpret_cast<float*>(smem + kKaWarps * C::kStages * C::kTile);
-    uint2* s_qf = reinterpret_cast<uint2*>(s_fold + C::kFold / 4);  // [NT][QP][G][4][32]: operand registers of the queries
+    uint4* s_qf = reinterpret_cast<uint4*>(s_fold + C::kFold / 4);  // [NT][QP][G][2][32]: operand registers of the queries, of two MMAs each
     float* s_max = reinterpret_cast<float*>(s_qf) + C::kOperands / 4;  // [warp][8 NT]
     float* s_sum = s_max + kKaWarps * 8 * NT;           // [warp][8 NT]
     float* s_most = s_sum + kKaWarps * 8 * NT;          // [G][8 NT]: largest |q|
@@ -308,7 +378,9 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
 
         // ---- the queries of this pass.  A warp prepares one group of 64 channels of every column (lane: column g, channels 16 j .. + 15);
         // the operand registers stay in shared memory, where every tile takes them from.
-        float q_sum[NT][2][G], mult[NT];  // sums of columns 2 j, 2 j + 1; factor of column g's scores, in units of log 2
+        float mult[NT];             // factor of column g's scores, in units of log 2
+        float q_sum[NT][2][kWide ? G : 1];  // fp32: sums over the groups' channels of columns 2 j, 2 j + 1
+        unsigned q_zero[NT][2];     // two-byte types: the sums of column g as operand registers, against the zero points
         int limit[NT][2], own_limit[NT];  // positions that the columns 2 j, 2 j + 1 see, and column g
         {
             float q[NT][16];
@@ -358,13 +430,15 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                 sum += __shfl_xor_sync(kFullMask, sum, 2);
                 if (j == 0) s_qsum[(nt * 8 + g) * G + warp] = sum * pow2(-24);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {  // MMA m takes the codes 2 (m % 2), + 1, + 4, + 5 of word m / 2
-                    const int c = (m >> 1) * 8 + (m & 1) * 2;
-                    uint2 hi, lo;
-                    split_half(q[nt][c], q[nt][c + 4], hi.x, lo.x);
-                    split_half(q[nt][c + 1] * 0.0625f, q[nt][c + 5] * 0.0625f, hi.y, lo.y);
-                    s_qf[(((nt * QP) * G + warp) * 4 + m) * 32 + lane] = hi;
-                    if (QP == 2) s_qf[(((nt * QP + QP - 1) * G + warp) * 4 + m) * 32 + lane] = lo;
+                for (int w = 0; w < 2; ++w) {  // MMA m takes the codes 2 (m % 2), + 1, + 4, + 5 of word m / 2
+                    const float* x = &q[nt][8 * w];
+                    uint4 hi, lo;
+                    split_half(x[0], x[4], hi.x, lo.x);
+                    split_half(x[1] * 0.0625f, x[5] * 0.0625f, hi.y, lo.y);
+                    split_half(x[2], x[6], hi.z, lo.z);
+                    split_half(x[3] * 0.0625f, x[7] * 0.0625f, hi.w, lo.w);
+                    s_qf[(((nt * QP) * G + warp) * 2 + w) * 32 + lane] = hi;
+                    if (QP == 2) s_qf[(((nt * QP + QP - 1) * G + warp) * 2 + w) * 32 + lane] = lo;
                 }
             }
             __syncthreads();
@@ -378,9 +452,28 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                 // what belongs to a column, for the lanes that hold it in the products' layout: columns 2 j, 2 j + 1
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) q_sum[nt][c][gr] = s_qsum[(nt * 8 + 2 * j + c) * G + gr];
                     limit[nt][c] = __shfl_sync(kFullMask, own_limit[nt], (2 * j + c) * 4);
+                    if constexpr (kWide) {
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) q_sum[nt][c][gr] = s_qsum[(nt * 8 + 2 * j + c) * G + gr];
+                    }
+                }
+                if constexpr (!kWide) {
+                    // k = 0..3 and 4..7 (and 8..15 for bf16): the sums of the groups, in two parts (four) that add up to 22 bits (32)
+                    float x[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) x[i] = 2 * (j & 1) + i < G ? s_qsum[(nt * 8 + g) * G + (2 * (j & 1) + i) % G] : 0.f;
+                    if (std::is_same<T, __half>::value) x[0] *= pow2(16), x[1] *= pow2(16);  // room for f16's second part; taken back below
+                    unsigned part[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        part[i] = KaPair<T>::pack(x[0], x[1]);
+                        const float2 f = KaPair<T>::unpack(part[i]);
+                        x[0] -= f.x, x[1] -= f.y;
+                    }
+                    const bool second = j >> 1;
+                    q_zero[nt][0] = second ? part[1] : part[0];
+                    q_zero[nt][1] = std::is_same<T, __half>::value ? 0u : (second ? part[3] : part[2]);
                 }
             }
         }
@@ -390,22 +483,24 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
         sees_all = min(sees_all, __shfl_xor_sync(kFullMask, sees_all, 1));
         sees_all = min(sees_all, __shfl_xor_sync(kFullMask, sees_all, 2));
 
-        float o[NT][G][4][4], zero_sum[NT][G], top[NT], weight_sum[NT];
+        // zero_sum: the zero points' part, of column g for every group (fp32), or as an MMA leaves it: row g % 4 (the group), columns 2 j, 2 j + 1
+        constexpr int Z = kWide ? G : 4;
+        float o[NT][G][4][4], zero_sum[NT][Z], top[NT], weight_sum[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             top[nt] = -INFINITY;
             weight_sum[nt] = 0.f;
 #pragma unroll
+            for (int i = 0; i < Z; ++i) zero_sum[nt][i] = 0.f;
+#pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                zero_sum[nt][gr] = 0.f;
 #pragma unroll
                 for (int m = 0; m < 4; ++m)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[nt][gr][m][i] = 0.f;
             }
         }
-        int unit = 1, unit_limit = 0;  // exponent field of the power of two that weights times scales are divided by; none yet
-        float shrink = pow2(126);
+        int unit = ka_least_unit<T>(), unit_limit = -1;  // exponent field of the scale that the values' sums are in units of; none yet
 
         for (; at < segment_end; at += kKaWarps) {
             const int tile = now.tile + (at - segment);
@@ -421,20 +516,34 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
 
             // ---- scores
             float s[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
             {
-                float ks[2][G], kz[2][G];
-                load_params<T, G>(params + g * (G * 2 * (int)sizeof(T)), ks[0], kz[0]);
-                load_params<T, G>(params + (g + 8) * (G * 2 * (int)sizeof(T)), ks[1], kz[1]);
                 constexpr int kUnit = D >= 128 ? 16 : 8, kVecs = D / 8 / kUnit, kWords = kUnit / 4;
                 unsigned a[kVecs][kWords], a8[kVecs][kWords];  // tokens g and g + 8
 #pragma unroll
                 for (int v = 0; v < kVecs; ++v) {
                     lds_words(codes + (v * 32 + lane) * kUnit, a[v]);
                     lds_words(codes + ((kVecs + v) * 32 + lane) * kUnit, a8[v]);
+                }
+                float ks[2][G], kz[2][G];
+                load_params<T, G>(params + g * (G * 2 * (int)sizeof(T)), ks[0], kz[0]);
+                load_params<T, G>(params + (g + 8) * (G * 2 * (int)sizeof(T)), ks[1], kz[1]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+                if constexpr (!kWide) {  // zero points times sums of the queries: one MMA, tokens x groups by groups x columns
+                    unsigned z[2][G > 1 ? 2 : 1];  // of tokens g and g + 8: groups 2 (j % 2) and the next
+                    lds_words(params + (g * G + (2 * (j & 1)) % G) * 4, z[0]);
+                    lds_words(params + ((g + 8) * G + (2 * (j & 1)) % G) * 4, z[1]);
+                    const unsigned a0 = __byte_perm(z[0][0], z[0][G > 1 ? 1 : 0], 0x7632), a1 = __byte_perm(z[1][0], z[1][G > 1 ? 1 : 0], 0x7632);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        ka_mma_params<T>(s[nt], a0, a1, a0, a1, q_zero[nt][0], q_zero[nt][1]);
+                        if (std::is_same<T, __half>::value) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[nt][i] *= pow2(-16);
+                        }
+                    }
                 }
                 float acc[NT][G][4];
 #pragma unroll
@@ -444,19 +553,27 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[nt][gr][i] = 0.f;
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {  // the groups' chains side by side: an MMA does not wait for the one before it
+                for (int w = 0; w < 2; ++w) {  // the groups' chains side by side: an MMA does not wait for the one before it
+                    uint4 b[NT][QP][G];
 #pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        const int v = gr / (kWords / 2), x = 2 * (gr % (kWords / 2)) + (m >> 1);
-                        const unsigned wa = a[v][x] >> (8 * (m & 1)), wb = a8[v][x] >> (8 * (m & 1));
-                        const unsigned a0 = wa & 0x000f000fu, a1 = wb & 0x000f000fu, a2 = wa & 0x00f000f0u, a3 = wb & 0x00f000f0u;
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int part = 0; part < QP; ++part)
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const uint2 b = s_qf[(((nt * QP + part) * G + gr) * 4 + m) * 32 + lane];
-                                ka_mma(acc[nt][gr], a0, a1, a2, a3, b.x, b.y);
-                            }
+                            for (int gr = 0; gr < G; ++gr) b[nt][part][gr] = s_qf[(((nt * QP + part) * G + gr) * 2 + w) * 32 + lane];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) {
+                            const int v = gr / (kWords / 2), x = 2 * (gr % (kWords / 2)) + w;
+                            const unsigned wa = a[v][x] >> (8 * m), wb = a8[v][x] >> (8 * m);
+                            const unsigned a0 = wa & 0x000f000fu, a1 = wb & 0x000f000fu, a2 = wa & 0x00f000f0u, a3 = wb & 0x00f000f0u;
+#pragma unroll
+                            for (int part = 0; part < QP; ++part)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+                                    ka_mma(acc[nt][gr], a0, a1, a2, a3, m ? b[nt][part][gr].z : b[nt][part][gr].x, m ? b[nt][part][gr].w : b[nt][part][gr].y);
+                        }
                     }
                 }
 #pragma unroll
@@ -464,45 +581,67 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            s[nt][i] = fmaf(ks[i >> 1][gr], acc[nt][gr][i], fmaf(kz[i >> 1][gr], q_sum[nt][i & 1][gr], s[nt][i]));
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (kWide) s[nt][i] = fmaf(kz[i >> 1][gr], q_sum[nt][i & 1][gr], s[nt][i]);
+                            s[nt][i] = fmaf(ks[i >> 1][gr], acc[nt][gr][i], s[nt][i]);
+                        }
             }
             const int first = tile * kKv4Tile;
             const bool edge = first + kKv4Tile > sees_all;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+                if (edge) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (edge && first + g + 8 * (i >> 1) >= limit[nt][i & 1]) s[nt][i] = -INFINITY;
+                    for (int i = 0; i < 4; ++i)
+                        if (first + g + 8 * (i >> 1) >= limit[nt][i & 1]) s[nt][i] = -INFINITY;
                 }
                 // from (tokens g, g + 8; columns 2 j, 2 j + 1) to (tokens 2 j, 2 j + 1, + 8, + 9; column g)
                 transpose8(s[nt][0], s[nt][1]);
                 transpose8(s[nt][2], s[nt][3]);
             }
 
-            // ---- scales and zero points of the values of the lane's four tokens
-            float vs[4][G], vz[4][G];
+            // ---- scales of the values of the lane's four tokens.  The sums are kept in units of a scale's power of two, so that f16 holds
+            // weights times scales, and the unit is raised when a scale is 2^4 times larger (2^11 for fp32).  The exponents' bits or'ed
+            // together are no smaller than the largest; only where that says so, it is looked for.
+            const unsigned char* v_params = params + kv4_param_bytes(D, sizeof(T));
+            unsigned sw[2][G];                          // two-byte types: pairs of tokens
+            float vs[4][kWide ? G : 1], vz[4][kWide ? G : 1];
+            bool larger;
+            if constexpr (!kWide) {
+                unsigned w[4][G], bits = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = 2 * j + (i & 1) + 8 * (i >> 1);
-                load_params<T, G>(params + kv4_param_bytes(D, sizeof(T)) + t * (G * 2 * (int)sizeof(T)), vs[i], vz[i]);
-                if (edge && first + t >= length) {  // behind the row's end anything may lie
+                for (int i = 0; i < 4; ++i) lds_words(v_params + (2 * j + (i & 1) + 8 * (i >> 1)) * (G * 4), w[i]);
 #pragma unroll
-                    for (int gr = 0; gr < G; ++gr) vs[i][gr] = vz[i][gr] = 0.f;
+                for (int gr = 0; gr < G; ++gr) sw[0][gr] = __byte_perm(w[0][gr], w[1][gr], 0x5410), sw[1][gr] = __byte_perm(w[2][gr], w[3][gr], 0x5410);
+                if (edge) {  // behind the row's end anything may lie
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const unsigned keep = ka_keep(first + 2 * j + 8 * x, length);
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) sw[x][gr] &= keep;
+                    }
                 }
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) bits |= sw[0][gr] | sw[1][gr];
+                larger = (int)((bits | bits >> 16) & KaPair<T>::kExponent) > unit_limit * (1 << KaPair<T>::kShift);
+            } else {
+                unsigned bits = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = 2 * j + (i & 1) + 8 * (i >> 1);
+                    load_params<T, G>(v_params + t * (G * 8), vs[i], vz[i]);
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        if (edge && first + t >= length) vs[i][gr] = vz[i][gr] = 0.f;
+                        bits |= __float_as_uint(vs[i][gr]);
+                    }
+                }
+                larger = (int)(bits >> 23) > unit_limit;
             }
-            // Weights times scales are divided by 2^(unit - 127): they stay below 2^15 as long as no scale's exponent passes unit + 13.
-            // The exponents' bits or'ed together are no smaller than the largest; only where that says so, it is looked for.
-            unsigned bits = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) bits |= __float_as_uint(vs[i][gr]);
-            const bool larger = (int)(bits >> 23) > unit_limit;
 
             // ---- running maximum; what has been summed is brought to it
             float corr[NT];
-            bool moved = larger;
+            bool moved = larger, poisoned = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float m = fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3]));
@@ -513,46 +652,148 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                 corr[nt] = exp2_approx((top[nt] - base) * mult[nt]);
                 moved |= m != top[nt];
                 top[nt] = m;
-                const float shift = base * mult[nt];
+                const float shift = 4.f - base * mult[nt];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    // fp32: the difference first, which is exact where it matters
-                    s[nt][i] = sizeof(T) == 4 ? exp2f((s[nt][i] - base) * mult[nt]) : exp2_approx(fmaf(s[nt][i], mult[nt], -shift));
+                    // weights of the two-byte types are 2^4 times as large, which gives small ones bits in f16.  fp32: the difference first,
+                    // which is exact where it matters
+                    s[nt][i] = kWide ? exp2f((s[nt][i] - base) * mult[nt]) : exp2_approx(fmaf(s[nt][i], mult[nt], shift));
                 }
             }
             if (__any_sync(kFullMask, moved)) {
-                int unit_now = unit;
+                float down = 1.f;
                 if (__any_sync(kFullMask, larger)) {
-                    unsigned largest = 0;
+                    int largest = 0;  // an exponent field; that of a NaN is no size: other columns may not see it
+                    if constexpr (!kWide) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) {
-                            const unsigned x = __float_as_uint(vs[i][gr]);
-                            largest = max(largest, x < 0x7f800000u ? x : 0u);  // a NaN is no size: other columns may not see it
+                        for (int i = 0; i < 4 * G; ++i) {
+                            const unsigned f = (sw[i / 2 / G][i / 2 % G] >> (16 * (i & 1)) & KaPair<T>::kExponent) >> KaPair<T>::kShift;
+                            if (f == KaPair<T>::kTop) poisoned = true;
+                            else largest = max(largest, (int)f);
                         }
-                    largest = max(largest, __shfl_xor_sync(kFullMask, largest, 1));
-                    largest = max(largest, __shfl_xor_sync(kFullMask, largest, 2));
-                    unit_now = max(unit, min((int)(largest >> 23), 253));
+                        poisoned = __any_sync(kFullMask, poisoned);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) {
+                                const int f = (int)(__float_as_uint(vs[i][gr]) >> 23);
+                                if (f < 255) largest = max(largest, min(f, 253));
+                            }
+                    }
+                    largest = __reduce_max_sync(kFullMask, largest);
+                    if (largest > unit) {
+                        down = pow2(max(unit - largest, -126));
+                        unit = largest;
+                    }
+                    unit_limit = min(unit + (kWide ? 11 : 3), 254);  // the exponent of a NaN is always beyond it
                 }
-                const float down = pow2(max(unit - unit_now, -126));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     weight_sum[nt] *= corr[nt];
-                    const float c0 = __shfl_sync(kFullMask, corr[nt], 8 * j) * down, c1 = __shfl_sync(kFullMask, corr[nt], 8 * j + 4) * down;
+                    const float k0 = __shfl_sync(kFullMask, corr[nt], 8 * j), k1 = __shfl_sync(kFullMask, corr[nt], 8 * j + 4);
+                    const float c0 = k0 * down, c1 = k1 * down;
+                    if constexpr (kWide) {
 #pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        zero_sum[nt][gr] *= corr[nt];
+                        for (int gr = 0; gr < G; ++gr) zero_sum[nt][gr] *= corr[nt];
+                    } else {
+                        zero_sum[nt][0] *= k0, zero_sum[nt][1] *= k1;
+                    }
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr)
 #pragma unroll
                         for (int m = 0; m < 4; ++m) {
                             o[nt][gr][m][0] *= c0, o[nt][gr][m][1] *= c1;
                             o[nt][gr][m][2] *= c0, o[nt][gr][m][3] *= c1;
                         }
+                }
+            }
+
+            // ---- weights times scales, in two halves; the zero points' part
+            unsigned hi[NT][G][2], lo[NT][G][2];
+            if constexpr (!kWide) {
+                unsigned scale[2][G];
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) scale[x][gr] = KaPair<T>::scales(sw[x][gr], unit);
+                if (std::is_same<T, __nv_bfloat16>::value && poisoned) {  // the shift of exponents does not do for a NaN
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) {
+                            const float2 f = KaPair<T>::unpack(sw[x][gr]);
+                            scale[x][gr] = pack_half(f.x * pow2(134 - unit), f.y * pow2(134 - unit));
+                        }
+                }
+                unsigned z[4], za[2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[i] = *reinterpret_cast<const unsigned*>(v_params + ((2 * j + (i & 1) + 8 * (i >> 1)) * G + g % G) * 4);
+                za[0] = __byte_perm(z[0], z[1], 0x7632), za[1] = __byte_perm(z[2], z[3], 0x7632);
+                if (edge) {  // nothing behind the row's end, and no NaN, which a weight of 0 would let through: its scale is a NaN too
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        unsigned keep = ka_keep(first + 2 * j + 8 * x, length);
+                        if ((za[x] & KaPair<T>::kExponent) == KaPair<T>::kExponent) keep &= 0xffff0000u;
+                        if ((za[x] >> 16 & KaPair<T>::kExponent) == KaPair<T>::kExponent) keep &= 0x0000ffffu;
+                        za[x] &= keep;
                     }
                 }
-                unit = unit_now;
-                unit_limit = unit + 13;
-                shrink = pow2(127 - unit);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    weight_sum[nt] += (s[nt][0] + s[nt][1]) + (s[nt][2] + s[nt][3]);
+                    unsigned ph[2], pl[2];
+                    split_half(s[nt][0], s[nt][1], ph[0], pl[0]);
+                    split_half(s[nt][2], s[nt][3], ph[1], pl[1]);
+                    if (std::is_same<T, __nv_bfloat16>::value) {  // operands of one type: the weights once more, as two bf16 (16 bits)
+                        unsigned bh[2], bl[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            bh[x] = KaPair<__nv_bfloat16>::pack(s[nt][2 * x], s[nt][2 * x + 1]);
+                            const float2 f = KaPair<__nv_bfloat16>::unpack(bh[x]);
+                            bl[x] = KaPair<__nv_bfloat16>::pack(s[nt][2 * x] - f.x, s[nt][2 * x + 1] - f.y);
+                        }
+                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, bl[0], bl[1]);
+                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, bh[0], bh[1]);
+                    } else {
+                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, pl[0], pl[1]);
+                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, ph[0], ph[1]);
+                    }
+                    if (edge) {  // what the column does not see may be a NaN
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const unsigned keep = ka_keep(first + 2 * j + 8 * x, own_limit[nt]);
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr] & keep, hi[nt][gr][x], lo[nt][gr][x]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr], hi[nt][gr][x], lo[nt][gr][x]);
+                    }
+                }
+            } else {
+                const float shrink = pow2(127 - unit);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    weight_sum[nt] += (s[nt][0] + s[nt][1]) + (s[nt][2] + s[nt][3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (edge && first + 2 * j + (i & 1) + 8 * (i >> 1) >= own_limit[nt]) {
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) vs[i][gr] = vz[i][gr] = 0.f;  // NT is 1: no other column of this lane
+                        }
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) zero_sum[nt][gr] = fmaf(s[nt][i], vz[i][gr], zero_sum[nt][gr]);
+                        s[nt][i] *= shrink;
+                    }
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        split_half(s[nt][0] * vs[0][gr], s[nt][1] * vs[1][gr], hi[nt][gr][0], lo[nt][gr][0]);
+                        split_half(s[nt][2] * vs[2][gr], s[nt][3] * vs[3][gr], hi[nt][gr][1], lo[nt][gr][1]);
+                    }
+                }
             }
 
             // ---- values
@@ -560,37 +801,6 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
             unsigned v[4][G];
 #pragma unroll
             for (int i = 0; i < 4; ++i) lds_words(codes + kv4_code_bytes(D) + (i * 32 + lane) * kUnit, v[i]);
-            unsigned hi[NT][G][2], lo[NT][G][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                weight_sum[nt] += (s[nt][0] + s[nt][1]) + (s[nt][2] + s[nt][3]);
-                auto weigh = [&](const float (&scale)[4][G], const float (&zero)[4][G]) {
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) zero_sum[nt][gr] = fmaf(s[nt][i], zero[i][gr], zero_sum[nt][gr]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] *= shrink;
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        split_half(s[nt][0] * scale[0][gr], s[nt][1] * scale[1][gr], hi[nt][gr][0], lo[nt][gr][0]);
-                        split_half(s[nt][2] * scale[2][gr], s[nt][3] * scale[3][gr], hi[nt][gr][1], lo[nt][gr][1]);
-                    }
-                };
-                if (edge) {  // what the column does not see may be a NaN, which a weight of 0 would let through
-                    float scale[4][G], zero[4][G];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool seen = first + 2 * j + (i & 1) + 8 * (i >> 1) < own_limit[nt];
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) scale[i][gr] = seen ? vs[i][gr] : 0.f, zero[i][gr] = seen ? vz[i][gr] : 0.f;
-                    }
-                    weigh(scale, zero);
-                } else {
-                    weigh(vs, vz);
-                }
-            }
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
                 unsigned a[4][4];
@@ -642,10 +852,12 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
         for (int nt = 0; nt < NT; ++nt) {
             weight_sum[nt] += __shfl_xor_sync(kFullMask, weight_sum[nt], 1);
             weight_sum[nt] += __shfl_xor_sync(kFullMask, weight_sum[nt], 2);
+            if constexpr (kWide) {
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-                zero_sum[nt][gr] += __shfl_xor_sync(kFullMask, zero_sum[nt][gr], 1);
-                zero_sum[nt][gr] += __shfl_xor_sync(kFullMask, zero_sum[nt][gr], 2);
+                for (int gr = 0; gr < G; ++gr) {
+                    zero_sum[nt][gr] += __shfl_xor_sync(kFullMask, zero_sum[nt][gr], 1);
+                    zero_sum[nt][gr] += __shfl_xor_sync(kFullMask, zero_sum[nt][gr], 2);
+                }
             }
             if (j == 0) {
                 const int c = (warp * NT + nt) * 8 + g;
@@ -654,7 +866,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
             }
         }
         __syncthreads();
-        const float grow = pow2(unit - 127);
+        const float grow = ka_unit_value<T>(unit);
         const long long slot = 2ll * blockIdx.x + (segment > begin ? 1 : 0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -668,7 +880,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                 // channel 8 g + i of a group at 8 i + g
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
-                    const float zero = __shfl_sync(kFullMask, zero_sum[nt][gr], (2 * j + c) * 4);
+                    const float zero = kWide ? __shfl_sync(kFullMask, zero_sum[nt][gr % Z], (2 * j + c) * 4) : __shfl_sync(kFullMask, zero_sum[nt][c], gr * 4 + j);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int m4 = (k >> 2) * 2 + (k & 1), half = (k >> 1) & 1;  // channel 8 g + k lies in these registers
