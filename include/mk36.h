@@ -462,6 +462,7 @@ typedef struct mk36_kv4_tokens {
     int64_t tokens; /* of each row, or of all rows with cu_tokens */
     int64_t k_row, k_token, k_head;
     int64_t v_row, v_token, v_head;
+    int32_t clear_rest; /* read: not 0 writes zeros behind the last row's tokens */
 } mk36_kv4_tokens;
 
 /* Quantises and writes them.  Of a group: zero = the least value, scale = (greatest - least) / 15 rounded to dtype, code =
@@ -470,7 +471,7 @@ typedef struct mk36_kv4_tokens {
  * outside the pool, behind the last row) are not written.  No two rows may hold the page that a token is written to. */
 MK36_API int mk36_kv4_append(const mk36_kv4_cache* cache, const mk36_kv4_tokens* tokens, void* stream);
 /* Reads them back, rounded once; tokens of a position below zero come back as zeros, those without a page in the pool as NaN, and
- * what lies behind the last row's tokens is left as it was. */
+ * what lies behind the last row's tokens is left as it was, or cleared with clear_rest. */
 MK36_API int mk36_kv4_read(const mk36_kv4_cache* cache, const mk36_kv4_tokens* tokens, void* stream);
 
 /* Attention of the last `tokens` tokens of every row over the row: q, out [rows, tokens, query_heads, head_dim] (out dense, q

@@ -27,6 +27,12 @@
 
 namespace mk36 {
 
+#ifndef KA_CTAS
+#define KA_CTAS 2
+#endif
+#ifndef KA_STEP
+#define KA_STEP 2
+#endif
 constexpr int kKaWarps = 4;
 constexpr int kKaThreads = kKaWarps * 32;
 constexpr int kKaMinTiles = 8;     // fewest tiles of a piece: two a warp
@@ -50,7 +56,9 @@ struct Kv4AttnParams {
 __host__ __device__ constexpr int ka_slot_floats(int d, int nt) { return 8 * nt * (d + 4); }
 
 // What their registers leave room for.
-__host__ __device__ constexpr int ka_ctas_per_sm(bool fp32, int nt) { return fp32 || nt == 2 ? 2 : 3; }
+__host__ __device__ constexpr int ka_ctas_per_sm(bool fp32, int nt) { return fp32 || nt == 2 ? 2 : KA_CTAS; }
+__host__ __device__ constexpr int ka_step(bool fp32, int nt) { return fp32 || nt == 2 ? 1 : KA_STEP; }
+
 
 template <typename T, int D, int NT>
 struct KaConfig {
@@ -63,10 +71,12 @@ struct KaConfig {
     static constexpr int kOperands = NT * kQParts * kGroups * 4 * 32 * 8;  // of the queries
     static constexpr int kStats = (kKaWarps * 8 * NT * 2 + 8 * NT * kGroups * 2) * 4;
     static constexpr int kRoom = 232448 / kCtas - 1024 - kFold - kOperands - kStats - 512;
+    // tiles a warp takes together: two where the registers allow it
+    static constexpr int kStep = ka_step(sizeof(T) == 4, NT);
     static constexpr int kMost = kRoom / (kKaWarps * kTile);
     static constexpr int kStages = kMost < 8 ? kMost : 8;
     static constexpr int kSmem = kKaWarps * kStages * kTile + kFold + kOperands + kStats + kKaWarps * kStages * 8;
-    static_assert(kStages >= 2, "no room for a ring");
+    static_assert(kStages > kStep, "no room for a ring");
 };
 
 __device__ __forceinline__ unsigned movmatrix(unsigned a) {
@@ -266,6 +276,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
     using C = KaConfig<T, D, NT>;
     constexpr int G = C::kGroups, QP = C::kQParts;
     constexpr bool kWide = sizeof(T) == 4;
+    constexpr int kStep = C::kStep;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int s_scan[kKaWarps], s_start[2], s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
@@ -485,11 +496,11 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
 
         // zero_sum: the zero points' part, of column g for every group (fp32), or as an MMA leaves it: row g % 4 (the group), columns 2 j, 2 j + 1
         constexpr int Z = kWide ? G : 4;
-        float o[NT][G][4][4], zero_sum[NT][Z], top[NT], weight_sum[NT];
+        float o[NT][G][4][4], zero_sum[NT][Z], top[NT], limit_top[NT], shift[NT], weight_sum[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            top[nt] = -INFINITY;
-            weight_sum[nt] = 0.f;
+            top[nt] = limit_top[nt] = -INFINITY;
+            shift[nt] = weight_sum[nt] = 0.f;
 #pragma unroll
             for (int i = 0; i < Z; ++i) zero_sum[nt][i] = 0.f;
 #pragma unroll
@@ -502,27 +513,46 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
         }
         int unit = ka_least_unit<T>(), unit_limit = -1;  // exponent field of the scale that the values' sums are in units of; none yet
 
-        for (; at < segment_end; at += kKaWarps) {
-            const int tile = now.tile + (at - segment);
-            if (!dead && !mbar_wait(&bars[stage], use & 1, &s_abort)) dead = true;
+        while (at < segment_end) {
+            // kStep tiles together: their chains of dependent instructions run side by side.  A tile that is not there counts as one that
+            // nothing is seen of.
+            const unsigned char* codes[kStep];
+            int first[kStep], count = 0;
+#pragma unroll
+            for (int u = 0; u < kStep; ++u) {
+                codes[u] = codes[0];
+                first[u] = 0x3fffff00;
+                if (u == 0 || at + u * kKaWarps < segment_end) {
+                    ++count;
+                    const int st = stage + u < C::kStages ? stage + u : stage + u - C::kStages;
+                    if (!dead && !mbar_wait(&bars[st], (use + (st < stage)) & 1, &s_abort)) dead = true;
+                    if (lost >> st & 1u) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) weight_sum[nt] = __uint_as_float(0x7fc00000u);
+                    }
+                    codes[u] = ring + st * C::kTile;
+                    first[u] = (now.tile + (at - segment) + u * kKaWarps) * kKv4Tile;
+                }
+            }
+            at += count * kKaWarps;
             dead = __any_sync(kFullMask, dead);
-            if (dead || (lost >> stage & 1u)) {
+            if (dead) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) weight_sum[nt] = __uint_as_float(0x7fc00000u);
+                continue;
             }
-            if (dead) continue;
-            const unsigned char* codes = ring + stage * C::kTile;
-            const unsigned char* params = codes + 2 * kv4_code_bytes(D);
 
             // ---- scores
-            float s[NT][4];
-            {
+            float s[kStep][NT][4];
+#pragma unroll
+            for (int u = 0; u < kStep; ++u) {
+                const unsigned char* params = codes[u] + 2 * kv4_code_bytes(D);
                 constexpr int kUnit = D >= 128 ? 16 : 8, kVecs = D / 8 / kUnit, kWords = kUnit / 4;
                 unsigned a[kVecs][kWords], a8[kVecs][kWords];  // tokens g and g + 8
 #pragma unroll
                 for (int v = 0; v < kVecs; ++v) {
-                    lds_words(codes + (v * 32 + lane) * kUnit, a[v]);
-                    lds_words(codes + ((kVecs + v) * 32 + lane) * kUnit, a8[v]);
+                    lds_words(codes[u] + (v * 32 + lane) * kUnit, a[v]);
+                    lds_words(codes[u] + ((kVecs + v) * 32 + lane) * kUnit, a8[v]);
                 }
                 float ks[2][G], kz[2][G];
                 load_params<T, G>(params + g * (G * 2 * (int)sizeof(T)), ks[0], kz[0]);
@@ -530,7 +560,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] = 0.f;
+                    for (int i = 0; i < 4; ++i) s[u][nt][i] = 0.f;
                 if constexpr (!kWide) {  // zero points times sums of the queries: one MMA, tokens x groups by groups x columns
                     unsigned z[2][G > 1 ? 2 : 1];  // of tokens g and g + 8: groups 2 (j % 2) and the next
                     lds_words(params + (g * G + (2 * (j & 1)) % G) * 4, z[0]);
@@ -538,10 +568,10 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                     const unsigned a0 = __byte_perm(z[0][0], z[0][G > 1 ? 1 : 0], 0x7632), a1 = __byte_perm(z[1][0], z[1][G > 1 ? 1 : 0], 0x7632);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        ka_mma_params<T>(s[nt], a0, a1, a0, a1, q_zero[nt][0], q_zero[nt][1]);
+                        ka_mma_params<T>(s[u][nt], a0, a1, a0, a1, q_zero[nt][0], q_zero[nt][1]);
                         if (std::is_same<T, __half>::value) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) s[nt][i] *= pow2(-16);
+                            for (int i = 0; i < 4; ++i) s[u][nt][i] *= pow2(-16);
                         }
                     }
                 }
@@ -582,83 +612,82 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            if constexpr (kWide) s[nt][i] = fmaf(kz[i >> 1][gr], q_sum[nt][i & 1][gr], s[nt][i]);
-                            s[nt][i] = fmaf(ks[i >> 1][gr], acc[nt][gr][i], s[nt][i]);
+                            if constexpr (kWide) s[u][nt][i] = fmaf(kz[i >> 1][gr], q_sum[nt][i & 1][gr], s[u][nt][i]);
+                            s[u][nt][i] = fmaf(ks[i >> 1][gr], acc[nt][gr][i], s[u][nt][i]);
                         }
             }
-            const int first = tile * kKv4Tile;
-            const bool edge = first + kKv4Tile > sees_all;
+            bool edge[kStep];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (edge) {
+            for (int u = 0; u < kStep; ++u) {
+                edge[u] = first[u] + kKv4Tile > sees_all;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (first + g + 8 * (i >> 1) >= limit[nt][i & 1]) s[nt][i] = -INFINITY;
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (edge[u]) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (first[u] + g + 8 * (i >> 1) >= limit[nt][i & 1]) s[u][nt][i] = -INFINITY;
+                    }
+                    // from (tokens g, g + 8; columns 2 j, 2 j + 1) to (tokens 2 j, 2 j + 1, + 8, + 9; column g)
+                    transpose8(s[u][nt][0], s[u][nt][1]);
+                    transpose8(s[u][nt][2], s[u][nt][3]);
                 }
-                // from (tokens g, g + 8; columns 2 j, 2 j + 1) to (tokens 2 j, 2 j + 1, + 8, + 9; column g)
-                transpose8(s[nt][0], s[nt][1]);
-                transpose8(s[nt][2], s[nt][3]);
             }
 
             // ---- scales of the values of the lane's four tokens.  The sums are kept in units of a scale's power of two, so that f16 holds
-            // weights times scales, and the unit is raised when a scale is 2^4 times larger (2^11 for fp32).  The exponents' bits or'ed
+            // weights times scales, and the unit is raised when a scale is 2^4 times larger (2^9 for fp32).  The exponents' bits or'ed
             // together are no smaller than the largest; only where that says so, it is looked for.
-            const unsigned char* v_params = params + kv4_param_bytes(D, sizeof(T));
-            unsigned sw[2][G];                          // two-byte types: pairs of tokens
-            float vs[4][kWide ? G : 1], vz[4][kWide ? G : 1];
-            bool larger;
-            if constexpr (!kWide) {
-                unsigned w[4][G], bits = 0;
+            unsigned sw[kStep][2][G];  // two-byte types: pairs of tokens
+            float vs[kStep][4][kWide ? G : 1], vz[kStep][4][kWide ? G : 1];
+            bool larger = false;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds_words(v_params + (2 * j + (i & 1) + 8 * (i >> 1)) * (G * 4), w[i]);
+            for (int u = 0; u < kStep; ++u) {
+                const unsigned char* v_params = codes[u] + 2 * kv4_code_bytes(D) + kv4_param_bytes(D, sizeof(T));
+                if constexpr (!kWide) {
+                    unsigned w[4][G], bits = 0;
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) sw[0][gr] = __byte_perm(w[0][gr], w[1][gr], 0x5410), sw[1][gr] = __byte_perm(w[2][gr], w[3][gr], 0x5410);
-                if (edge) {  // behind the row's end anything may lie
+                    for (int i = 0; i < 4; ++i) lds_words(v_params + (2 * j + (i & 1) + 8 * (i >> 1)) * (G * 4), w[i]);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const unsigned keep = ka_keep(first + 2 * j + 8 * x, length);
+                    for (int gr = 0; gr < G; ++gr) sw[u][0][gr] = __byte_perm(w[0][gr], w[1][gr], 0x5410), sw[u][1][gr] = __byte_perm(w[2][gr], w[3][gr], 0x5410);
+                    if (edge[u]) {  // behind the row's end anything may lie
 #pragma unroll
-                        for (int gr = 0; gr < G; ++gr) sw[x][gr] &= keep;
+                        for (int x = 0; x < 2; ++x) {
+                            const unsigned keep = ka_keep(first[u] + 2 * j + 8 * x, length);
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) sw[u][x][gr] &= keep;
+                        }
                     }
-                }
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) bits |= sw[0][gr] | sw[1][gr];
-                larger = (int)((bits | bits >> 16) & KaPair<T>::kExponent) > unit_limit * (1 << KaPair<T>::kShift);
-            } else {
-                unsigned bits = 0;
+                    for (int gr = 0; gr < G; ++gr) bits |= sw[u][0][gr] | sw[u][1][gr];
+                    larger |= (int)((bits | bits >> 16) & KaPair<T>::kExponent) > unit_limit * (1 << KaPair<T>::kShift);
+                } else {
+                    unsigned bits = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = 2 * j + (i & 1) + 8 * (i >> 1);
-                    load_params<T, G>(v_params + t * (G * 8), vs[i], vz[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        const int t = 2 * j + (i & 1) + 8 * (i >> 1);
+                        load_params<T, G>(v_params + t * (G * 8), vs[u][i], vz[u][i]);
 #pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        if (edge && first + t >= length) vs[i][gr] = vz[i][gr] = 0.f;
-                        bits |= __float_as_uint(vs[i][gr]);
+                        for (int gr = 0; gr < G; ++gr) {
+                            if (edge[u] && first[u] + t >= length) vs[u][i][gr] = vz[u][i][gr] = 0.f;
+                            bits |= __float_as_uint(vs[u][i][gr]);
+                        }
                     }
+                    larger |= (int)(bits >> 23) > unit_limit;
                 }
-                larger = (int)(bits >> 23) > unit_limit;
             }
 
-            // ---- running maximum; what has been summed is brought to it
-            float corr[NT];
+            // ---- maximum.  Weights are taken relative to `top`, which follows the maximum only when that is 2^4 times larger: then, and not
+            // with every tile, what has been summed is brought to the new one.
+            float most[NT];
             bool moved = larger, poisoned = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float m = fmaxf(fmaxf(s[nt][0], s[nt][1]), fmaxf(s[nt][2], s[nt][3]));
+                float m = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < kStep; ++u) m = fmaxf(m, fmaxf(fmaxf(s[u][nt][0], s[u][nt][1]), fmaxf(s[u][nt][2], s[u][nt][3])));
                 m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 2));
-                m = fmaxf(m, top[nt]);
-                const float base = m == -INFINITY ? 0.f : m;
-                corr[nt] = exp2_approx((top[nt] - base) * mult[nt]);
-                moved |= m != top[nt];
-                top[nt] = m;
-                const float shift = 4.f - base * mult[nt];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // weights of the two-byte types are 2^4 times as large, which gives small ones bits in f16.  fp32: the difference first,
-                    // which is exact where it matters
-                    s[nt][i] = kWide ? exp2f((s[nt][i] - base) * mult[nt]) : exp2_approx(fmaf(s[nt][i], mult[nt], shift));
-                }
+                most[nt] = m;
+                moved |= m > limit_top[nt];
             }
             if (__any_sync(kFullMask, moved)) {
                 float down = 1.f;
@@ -666,18 +695,18 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                     int largest = 0;  // an exponent field; that of a NaN is no size: other columns may not see it
                     if constexpr (!kWide) {
 #pragma unroll
-                        for (int i = 0; i < 4 * G; ++i) {
-                            const unsigned f = (sw[i / 2 / G][i / 2 % G] >> (16 * (i & 1)) & KaPair<T>::kExponent) >> KaPair<T>::kShift;
+                        for (int i = 0; i < kStep * 4 * G; ++i) {
+                            const unsigned f = (sw[i / 4 / G][i / 2 / G % 2][i / 2 % G] >> (16 * (i & 1)) & KaPair<T>::kExponent) >> KaPair<T>::kShift;
                             if (f == KaPair<T>::kTop) poisoned = true;
                             else largest = max(largest, (int)f);
                         }
                         poisoned = __any_sync(kFullMask, poisoned);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < kStep * 4; ++i)
 #pragma unroll
                             for (int gr = 0; gr < G; ++gr) {
-                                const int f = (int)(__float_as_uint(vs[i][gr]) >> 23);
+                                const int f = (int)(__float_as_uint(vs[i / 4][i % 4][gr]) >> 23);
                                 if (f < 255) largest = max(largest, min(f, 253));
                             }
                     }
@@ -686,16 +715,21 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                         down = pow2(max(unit - largest, -126));
                         unit = largest;
                     }
-                    unit_limit = min(unit + (kWide ? 11 : 3), 254);  // the exponent of a NaN is always beyond it
+                    unit_limit = min(unit + (kWide ? 8 : 3), 254);  // the exponent of a NaN is always beyond it
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    weight_sum[nt] *= corr[nt];
-                    const float k0 = __shfl_sync(kFullMask, corr[nt], 8 * j), k1 = __shfl_sync(kFullMask, corr[nt], 8 * j + 4);
+                    const float m = fmaxf(top[nt], most[nt]);
+                    const float corr = m == -INFINITY ? 0.f : exp2f((top[nt] - m) * mult[nt]);  // nothing has been summed without a maximum
+                    top[nt] = m;
+                    limit_top[nt] = m == -INFINITY ? m : m + 4.f / mult[nt];
+                    shift[nt] = m == -INFINITY ? 0.f : -m * mult[nt];
+                    weight_sum[nt] *= corr;
+                    const float k0 = __shfl_sync(kFullMask, corr, 8 * j), k1 = __shfl_sync(kFullMask, corr, 8 * j + 4);
                     const float c0 = k0 * down, c1 = k1 * down;
                     if constexpr (kWide) {
 #pragma unroll
-                        for (int gr = 0; gr < G; ++gr) zero_sum[nt][gr] *= corr[nt];
+                        for (int gr = 0; gr < G; ++gr) zero_sum[nt][gr] *= corr;
                     } else {
                         zero_sum[nt][0] *= k0, zero_sum[nt][1] *= k1;
                     }
@@ -709,142 +743,157 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D, NT>::kCtas) kv4_att
                 }
             }
 
+            // fp32: the difference first, which is exact where it matters
+#pragma unroll
+            for (int u = 0; u < kStep; ++u)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[u][nt][i] = kWide ? exp2f((s[u][nt][i] - (top[nt] == -INFINITY ? 0.f : top[nt])) * mult[nt]) : exp2_approx(fmaf(s[u][nt][i], mult[nt], shift[nt]));
+
             // ---- weights times scales, in two halves; the zero points' part
-            unsigned hi[NT][G][2], lo[NT][G][2];
-            if constexpr (!kWide) {
-                unsigned scale[2][G];
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) scale[x][gr] = KaPair<T>::scales(sw[x][gr], unit);
-                if (std::is_same<T, __nv_bfloat16>::value && poisoned) {  // the shift of exponents does not do for a NaN
+            for (int u = 0; u < kStep; ++u) {
+                const unsigned char* v_params = codes[u] + 2 * kv4_code_bytes(D) + kv4_param_bytes(D, sizeof(T));
+                unsigned hi[NT][G][2], lo[NT][G][2];
+                if constexpr (!kWide) {
+                    unsigned scale[2][G];
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
-                        for (int gr = 0; gr < G; ++gr) {
-                            const float2 f = KaPair<T>::unpack(sw[x][gr]);
-                            scale[x][gr] = pack_half(f.x * pow2(134 - unit), f.y * pow2(134 - unit));
-                        }
-                }
-                unsigned z[4], za[2];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = *reinterpret_cast<const unsigned*>(v_params + ((2 * j + (i & 1) + 8 * (i >> 1)) * G + g % G) * 4);
-                za[0] = __byte_perm(z[0], z[1], 0x7632), za[1] = __byte_perm(z[2], z[3], 0x7632);
-                if (edge) {  // nothing behind the row's end, and no NaN, which a weight of 0 would let through: its scale is a NaN too
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        unsigned keep = ka_keep(first + 2 * j + 8 * x, length);
-                        if ((za[x] & KaPair<T>::kExponent) == KaPair<T>::kExponent) keep &= 0xffff0000u;
-                        if ((za[x] >> 16 & KaPair<T>::kExponent) == KaPair<T>::kExponent) keep &= 0x0000ffffu;
-                        za[x] &= keep;
-                    }
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    weight_sum[nt] += (s[nt][0] + s[nt][1]) + (s[nt][2] + s[nt][3]);
-                    unsigned ph[2], pl[2];
-                    split_half(s[nt][0], s[nt][1], ph[0], pl[0]);
-                    split_half(s[nt][2], s[nt][3], ph[1], pl[1]);
-                    if (std::is_same<T, __nv_bfloat16>::value) {  // operands of one type: the weights once more, as two bf16 (16 bits)
-                        unsigned bh[2], bl[2];
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            bh[x] = KaPair<__nv_bfloat16>::pack(s[nt][2 * x], s[nt][2 * x + 1]);
-                            const float2 f = KaPair<__nv_bfloat16>::unpack(bh[x]);
-                            bl[x] = KaPair<__nv_bfloat16>::pack(s[nt][2 * x] - f.x, s[nt][2 * x + 1] - f.y);
-                        }
-                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, bl[0], bl[1]);
-                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, bh[0], bh[1]);
-                    } else {
-                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, pl[0], pl[1]);
-                        ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, ph[0], ph[1]);
-                    }
-                    if (edge) {  // what the column does not see may be a NaN
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const unsigned keep = ka_keep(first + 2 * j + 8 * x, own_limit[nt]);
-#pragma unroll
-                            for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr] & keep, hi[nt][gr][x], lo[nt][gr][x]);
-                        }
-                    } else {
+                        for (int gr = 0; gr < G; ++gr) scale[x][gr] = KaPair<T>::scales(sw[u][x][gr], unit);
+                    if (std::is_same<T, __nv_bfloat16>::value && poisoned) {  // the shift of exponents does not do for a NaN
 #pragma unroll
                         for (int x = 0; x < 2; ++x)
 #pragma unroll
-                            for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr], hi[nt][gr][x], lo[nt][gr][x]);
+                            for (int gr = 0; gr < G; ++gr) {
+                                const float2 f = KaPair<T>::unpack(sw[u][x][gr]);
+                                scale[x][gr] = pack_half(f.x * pow2(134 - unit), f.y * pow2(134 - unit));
+                            }
                     }
-                }
-            } else {
-                const float shrink = pow2(127 - unit);
+                    unsigned z[4], za[2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    weight_sum[nt] += (s[nt][0] + s[nt][1]) + (s[nt][2] + s[nt][3]);
+                    for (int i = 0; i < 4; ++i) z[i] = *reinterpret_cast<const unsigned*>(v_params + ((2 * j + (i & 1) + 8 * (i >> 1)) * G + g % G) * 4);
+                    za[0] = __byte_perm(z[0], z[1], 0x7632), za[1] = __byte_perm(z[2], z[3], 0x7632);
+                    if (edge[u]) {  // nothing behind the row's end, and no NaN, which a weight of 0 would let through: its scale is a NaN too
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (edge && first + 2 * j + (i & 1) + 8 * (i >> 1) >= own_limit[nt]) {
+                        for (int x = 0; x < 2; ++x) {
+                            unsigned keep = ka_keep(first[u] + 2 * j + 8 * x, length);
+                            if ((za[x] & KaPair<T>::kExponent) == KaPair<T>::kExponent) keep &= 0xffff0000u;
+                            if ((za[x] >> 16 & KaPair<T>::kExponent) == KaPair<T>::kExponent) keep &= 0x0000ffffu;
+                            za[x] &= keep;
+                        }
+                    }
 #pragma unroll
-                            for (int gr = 0; gr < G; ++gr) vs[i][gr] = vz[i][gr] = 0.f;  // NT is 1: no other column of this lane
+                    for (int nt = 0; nt < NT; ++nt) {
+                        weight_sum[nt] += (s[u][nt][0] + s[u][nt][1]) + (s[u][nt][2] + s[u][nt][3]);
+                        unsigned ph[2], pl[2];
+                        split_half(s[u][nt][0], s[u][nt][1], ph[0], pl[0]);
+                        split_half(s[u][nt][2], s[u][nt][3], ph[1], pl[1]);
+                        if (std::is_same<T, __nv_bfloat16>::value) {  // operands of one type: the weights once more, as two bf16 (16 bits)
+                            unsigned bh[2], bl[2];
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                bh[x] = KaPair<__nv_bfloat16>::pack(s[u][nt][2 * x], s[u][nt][2 * x + 1]);
+                                const float2 f = KaPair<__nv_bfloat16>::unpack(bh[x]);
+                                bl[x] = KaPair<__nv_bfloat16>::pack(s[u][nt][2 * x] - f.x, s[u][nt][2 * x + 1] - f.y);
+                            }
+                            ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, bl[0], bl[1]);
+                            ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, bh[0], bh[1]);
+                        } else {
+                            ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, pl[0], pl[1]);
+                            ka_mma_params<T>(*reinterpret_cast<float(*)[4]>(zero_sum[nt]), za[0], 0u, za[1], 0u, ph[0], ph[1]);
+                        }
+                        if (edge[u]) {  // what the column does not see may be a NaN
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const unsigned keep = ka_keep(first[u] + 2 * j + 8 * x, own_limit[nt]);
+#pragma unroll
+                                for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr] & keep, hi[nt][gr][x], lo[nt][gr][x]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr], hi[nt][gr][x], lo[nt][gr][x]);
+                        }
+                    }
+                } else {
+                    const float shrink = pow2(127 - unit);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        weight_sum[nt] += (s[u][nt][0] + s[u][nt][1]) + (s[u][nt][2] + s[u][nt][3]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (edge[u] && first[u] + 2 * j + (i & 1) + 8 * (i >> 1) >= own_limit[nt]) {
+#pragma unroll
+                                for (int gr = 0; gr < G; ++gr) vs[u][i][gr] = vz[u][i][gr] = 0.f;  // NT is 1: no other column of this lane
+                            }
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) zero_sum[nt][gr] = fmaf(s[u][nt][i], vz[u][i][gr], zero_sum[nt][gr]);
+                            s[u][nt][i] *= shrink;
                         }
 #pragma unroll
-                        for (int gr = 0; gr < G; ++gr) zero_sum[nt][gr] = fmaf(s[nt][i], vz[i][gr], zero_sum[nt][gr]);
-                        s[nt][i] *= shrink;
+                        for (int gr = 0; gr < G; ++gr) {
+                            split_half(s[u][nt][0] * vs[u][0][gr], s[u][nt][1] * vs[u][1][gr], hi[nt][gr][0], lo[nt][gr][0]);
+                            split_half(s[u][nt][2] * vs[u][2][gr], s[u][nt][3] * vs[u][3][gr], hi[nt][gr][1], lo[nt][gr][1]);
+                        }
                     }
+                }
+
+                // ---- values
+                constexpr int kUnit = D / 16;
+                unsigned v[4][G];
 #pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        split_half(s[nt][0] * vs[0][gr], s[nt][1] * vs[1][gr], hi[nt][gr][0], lo[nt][gr][0]);
-                        split_half(s[nt][2] * vs[2][gr], s[nt][3] * vs[3][gr], hi[nt][gr][1], lo[nt][gr][1]);
+                for (int i = 0; i < 4; ++i) lds_words(codes[u] + kv4_code_bytes(D) + (i * 32 + lane) * kUnit, v[i]);
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    unsigned a[4][4];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {  // rows g and g + 8: channels 8 g + c and 8 g + c + 2, c = 0, 1 (x 16), 4, 5 (x 16)
+                        const unsigned pick = m < 2 ? 0x5410u : 0x7632u, mask = m & 1 ? 0x00f000f0u : 0x000f000fu;
+                        const unsigned near = __byte_perm(v[0][gr], v[1][gr], pick), far = __byte_perm(v[2][gr], v[3][gr], pick);
+                        a[m][0] = near & mask, a[m][1] = near >> 8 & mask, a[m][2] = far & mask, a[m][3] = far >> 8 & mask;
+                    }
+                    if (sizeof(T) == 4) {  // chains of two, added up in fp32: the tensor core cuts off where an addition rounds
+                        float acc[NT][4][4];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) acc[nt][m][i] = 0.f;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) ka_mma(acc[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][gr][0], lo[nt][gr][1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) ka_mma(acc[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][gr][0], hi[nt][gr][1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) add_tile(o[nt][gr][m], acc[nt][m]);
+                    } else {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) ka_mma(o[nt][gr][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][gr][0], lo[nt][gr][1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) ka_mma(o[nt][gr][m], a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][gr][0], hi[nt][gr][1]);
                     }
                 }
             }
 
-            // ---- values
-            constexpr int kUnit = D / 16;
-            unsigned v[4][G];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) lds_words(codes + kv4_code_bytes(D) + (i * 32 + lane) * kUnit, v[i]);
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-                unsigned a[4][4];
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {  // rows g and g + 8: channels 8 g + c and 8 g + c + 2, c = 0, 1 (x 16), 4, 5 (x 16)
-                    const unsigned pick = m < 2 ? 0x5410u : 0x7632u, mask = m & 1 ? 0x00f000f0u : 0x000f000fu;
-                    const unsigned near = __byte_perm(v[0][gr], v[1][gr], pick), far = __byte_perm(v[2][gr], v[3][gr], pick);
-                    a[m][0] = near & mask, a[m][1] = near >> 8 & mask, a[m][2] = far & mask, a[m][3] = far >> 8 & mask;
-                }
-                if (sizeof(T) == 4) {  // chains of two, added up in fp32: the tensor core cuts off where an addition rounds
-                    float acc[NT][4][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[nt][m][i] = 0.f;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) ka_mma(acc[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][gr][0], lo[nt][gr][1]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) ka_mma(acc[nt][m], a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][gr][0], hi[nt][gr][1]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) add_tile(o[nt][gr][m], acc[nt][m]);
-                } else {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) ka_mma(o[nt][gr][m], a[m][0], a[m][1], a[m][2], a[m][3], lo[nt][gr][0], lo[nt][gr][1]);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) ka_mma(o[nt][gr][m], a[m][0], a[m][1], a[m][2], a[m][3], hi[nt][gr][0], hi[nt][gr][1]);
-                }
+            __syncwarp();  // every lane has read the stages
+            for (int u = 0; u < count; ++u) {
+                request(stage);
+                if (++stage == C::kStages) stage = 0, ++use;
             }
-
-            __syncwarp();  // every lane has read the stage
-            request(stage);
-            if (++stage == C::kStages) stage = 0, ++use;
         }
 
         // ---- the end of a segment: the warps' sums meet

@@ -21,6 +21,8 @@ struct Kv4TokenParams {
     long long tokens, total;
     long long k_row, k_token, k_head, v_row, v_token, v_head;  // elements
     int wide;  // 1: every eight channels lie on a 16-byte boundary
+    int cta_tokens;
+    int clear;  // read: zeros behind the last row's tokens
     FastDiv per_row;
 };
 
@@ -47,54 +49,55 @@ __device__ __forceinline__ bool kv4_place(const Kv4TokenParams& p, long long i, 
     return true;
 }
 
+// Eight channels as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool wide, float (&f)[8]) {
+__device__ __forceinline__ Chunk8<T> load8(const T* p, bool wide) {
+    if (wide) return load_chunk8<T>(p);
+    Chunk8<T> c;
+    T* x = reinterpret_cast<T*>(&c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+    return c;
+}
+__device__ __forceinline__ const uint4& raw_of(const Chunk8<float>& c) { return c.lo; }
+template <typename T>
+__device__ __forceinline__ const uint4& raw_of(const Chunk8<T>& c) { return c.raw; }
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool wide, const Chunk8<T>& c) {
     if (wide) {
-        unpack8(load_chunk8<T>(p), f);
+        *reinterpret_cast<Chunk8<T>*>(p) = c;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_float<T>(p[i]);
+        for (int i = 0; i < 8; ++i) p[i] = reinterpret_cast<const T*>(&c)[i];
     }
 }
 
-__device__ __forceinline__ void store8(__nv_bfloat16* p, bool wide, const float (&f)[8]) {
-    if (wide) {
-        uint4 r;
-        unsigned* w = &r.x;
+// zero + code * scale, rounded once.  In two-byte types two at a time: 0x..0n or'ed to a power of two is that plus n, and a fused
+// product and sum of the types' own rounds once.
+template <typename T2>
+__device__ __forceinline__ void dequantise_pairs(unsigned word, unsigned param, unsigned power, uint4& out) {
+    const unsigned scale = __byte_perm(param, param, 0x1010), zero = __byte_perm(param, param, 0x3232);
+    unsigned n[4];  // codes i and i + 4
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const unsigned*>(&h);
-        }
-        *reinterpret_cast<uint4*>(p) = r;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = __float2bfloat16_rn(f[i]);
+    for (int i = 0; i < 4; ++i) {
+        const unsigned x = (word >> (4 * i) & 0x000f000fu) | power;
+        const T2 v = __hfma2(__hsub2(*reinterpret_cast<const T2*>(&x), *reinterpret_cast<const T2*>(&power)), *reinterpret_cast<const T2*>(&scale),
+                             *reinterpret_cast<const T2*>(&zero));
+        n[i] = *reinterpret_cast<const unsigned*>(&v);
     }
+    out = make_uint4(__byte_perm(n[0], n[1], 0x5410), __byte_perm(n[2], n[3], 0x5410), __byte_perm(n[0], n[1], 0x7632), __byte_perm(n[2], n[3], 0x7632));
 }
-__device__ __forceinline__ void store8(__half* p, bool wide, const float (&f)[8]) {
-    if (wide) {
-        uint4 r;
-        unsigned* w = &r.x;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const unsigned*>(&h);
-        }
-        *reinterpret_cast<uint4*>(p) = r;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = __float2half_rn(f[i]);
-    }
+__device__ __forceinline__ void dequantise(unsigned word, const Kv4Param<__nv_bfloat16>& p, Chunk8<__nv_bfloat16>& out) {
+    dequantise_pairs<__nv_bfloat162>(word, p.raw, 0x43004300u, out.raw);  // 128
 }
-__device__ __forceinline__ void store8(float* p, bool wide, const float (&f)[8]) {
-    if (wide) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
+__device__ __forceinline__ void dequantise(unsigned word, const Kv4Param<__half>& p, Chunk8<__half>& out) {
+    dequantise_pairs<__half2>(word, p.raw, 0x64006400u, out.raw);  // 1024
+}
+__device__ __forceinline__ void dequantise(unsigned word, const Kv4Param<float>& p, Chunk8<float>& out) {
+    float* f = reinterpret_cast<float*>(&out);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = f[i];
-    }
+    for (int i = 0; i < 8; ++i) f[i] = fmaf((float)(word >> (4 * i) & 15u), p.scale, p.zero);
 }
 
 // (high - low) / 15 rounded once to T, in fp64 throughout: the difference of two values of T is exact there or off by a part in
@@ -130,79 +133,80 @@ __device__ __noinline__ unsigned code_exact(float x, float zero, float scale) {
     return n > 0.0 ? (n < 15.0 ? (unsigned)n : 15u) : 0u;
 }
 
-// y = (x - zero) * (1 / scale) in fp32 is off by less than 2e-5 for codes up to 16: the difference and the product are off by
-// 2^-24 each, the reciprocal by 2^-23.
-__device__ __forceinline__ unsigned code_of(float x, float zero, float scale, float inv) {
-    const float y = (x - zero) * inv;
-    const float n = rintf(y);
-    if (!(fabsf(y - n) < 0.4999f)) return code_exact(x, zero, scale);
-    return n > 0.0f ? (n < 15.0f ? (unsigned)n : 15u) : 0u;
+// Values in registers: an array passed by its address would be stored to memory by every thread, called or not.
+__device__ __noinline__ unsigned four_exact(float4 x, float zero, float scale) {
+    return code_exact(x.x, zero, scale) | code_exact(x.y, zero, scale) << 4 | code_exact(x.z, zero, scale) << 8 | code_exact(x.w, zero, scale) << 12;
+}
+__device__ __forceinline__ unsigned codes_exact(const float (&x)[8], float zero, float scale) {
+    return four_exact(make_float4(x[0], x[1], x[2], x[3]), zero, scale) | four_exact(make_float4(x[4], x[5], x[6], x[7]), zero, scale) << 16;
 }
 
+constexpr float kRoundUp = 12582912.0f;  // 1.5 * 2^23: added, it rounds to a whole number, halves to even, and leaves that in the low bits
+
+// Whole numbers below 16, as floats, to a word of eight half bytes: sums of four are exact.
+__device__ __forceinline__ unsigned pack_codes(const float (&n)[8]) {
+    const float low = fmaf(n[3], 4096.0f, fmaf(n[2], 256.0f, fmaf(n[1], 16.0f, n[0]))), high = fmaf(n[7], 4096.0f, fmaf(n[6], 256.0f, fmaf(n[5], 16.0f, n[4])));
+    return __byte_perm(__float_as_uint(low + kRoundUp), __float_as_uint(high + kRoundUp), 0x5410);
+}
+
+// Codes of two-byte values.  n = the whole number nearest to (x - zero) / scale by way of an approximate reciprocal is right, or next to
+// it where the quotient lies at a border: what is left, r = (x - zero) - n scale, says so, because it is exact.  (n scale has 15
+// bits at most; x - zero has 24 and is off by e at most half its last place; half the scale is a multiple of that place.)
+// Values half way between two codes are common, one in some hundred of bf16: about every second warp has one.
 template <typename T>
-__device__ __forceinline__ void write_param(unsigned char* p, float scale, float zero, bool fine) {
-    if (sizeof(T) == 4) {
-        *reinterpret_cast<float2*>(p) = make_float2(scale, zero);
-    } else {
-        constexpr unsigned kNan = std::is_same<T, __half>::value ? 0x7e007e00u : 0x7fc07fc0u;
-        T two[2] = {from_float<T>(scale), from_float<T>(zero)};
-        *reinterpret_cast<unsigned*>(p) = fine ? *reinterpret_cast<const unsigned*>(two) : kNan;
+__device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, float high, float scale, const T*) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    // scales of a few units of the smallest number, whose quotients may be far beyond 15, and what the reciprocal does not hold
+    if (!(scale >= 1e-30f && (high - zero) * inv <= 15.4f)) return codes_exact(x, zero, scale);
+    const float half = 0.5f * scale;
+    float n[8], r[8];
+    bool border = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float d = x[i] - zero;
+        n[i] = fmaf(d, inv, kRoundUp) - kRoundUp;
+        r[i] = fmaf(-n[i], scale, d);
+        border |= fabsf(r[i]) >= half;
     }
-}
-
-// One of 2 * kv_heads * D / 8 pieces of a token: keys of all heads, then values.
-template <typename T, int D>
-struct Kv4Piece {
-    const T* dense;             // its channels in k or v
-    unsigned char *word, *param;  // its codes and its group's parameters in the cache
-    bool placed, in_pool;
-};
-
-template <typename T, int D>
-__device__ __forceinline__ bool kv4_piece(const Kv4TokenParams& p, long long unit, int pieces, Kv4Piece<T, D>& out) {
-    const long long i = unit / pieces;
-    int piece = (int)(unit - i * pieces);
-    int row, local, position;
-    if (i >= p.total || !kv4_place(p, i, row, local, position)) return false;
-    const bool is_k = piece < pieces / 2;
-    if (!is_k) piece -= pieces / 2;
-    const int head = piece / (D / 8), c = piece % (D / 8) * 8;
-    const long long at = is_k ? (p.cu ? i * p.k_token : row * p.k_row + local * p.k_token) + head * p.k_head
-                              : (p.cu ? i * p.v_token : row * p.v_row + local * p.v_token) + head * p.v_head;
-    out.dense = reinterpret_cast<const T*>(is_k ? p.k : p.v) + at + c;
-    out.placed = position >= 0;
-    out.in_pool = false;
-    out.word = out.param = nullptr;
-    if (out.placed) {
-        int slot, inner;
-        fdivmod(position / kKv4Tile, p.cache.tiles_per_page, slot, inner);
-        const long long page = p.cache.table[(long long)row * p.cache.row_pages + slot];
-        if (page >= 0 && page < p.cache.pages) {
-            out.in_pool = true;
-            unsigned char* tile = p.cache.pool + ((page * p.cache.kv_heads + head) * (long long)p.cache.tiles_per_page.d + inner) * p.cache.tile_bytes;
-            const int t = position % kKv4Tile;
-            out.word = tile + (is_k ? kv4_key_word<D>(t, c) : kv4_value_word<D>(t, c));
-            out.param = tile + 2 * kv4_code_bytes(D) + (is_k ? 0 : kv4_param_bytes(D, sizeof(T))) + (t * (D / kKv4Group) + c / kKv4Group) * 2 * sizeof(T);
+    if (border) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (fabsf(r[i]) >= half) {
+                const float d = x[i] - zero, part = x[i] - d, e = (part - zero) + (x[i] - (d + part));  // what the difference lost
+                const float way = copysignf(1.0f, r[i]), over = fmaf(way, e, fabsf(r[i]) - half);       // its sign is exact
+                const bool odd = __float_as_uint(n[i] + kRoundUp) & 1u;
+                if (over > 0.0f || (over == 0.0f && odd)) n[i] += way;
+            }
         }
     }
-    return true;
+    return pack_codes(n);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4TokenParams p) {
-    const int pieces = 2 * p.cache.kv_heads * (D / 8);
-    const long long unit = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    Kv4Piece<T, D> piece;
-    // the eight threads of a group take the same way; the warp stays together for the shuffles
-    const bool go = kv4_piece<T, D>(p, unit, pieces, piece) && piece.in_pool;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (go) load8<T>(piece.dense, p.wide != 0, f);
-    float low = f[0], high = f[0], sum = 0.f;
+// Codes of fp32 values: neither the difference nor the product is exact, so near a border fp64 decides.  The quotient is off by less than
+// 2e-5: difference, product and reciprocal by 2^-23 or less each.
+__device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, float high, float scale, const float*) {
+    const float inv = 1.0f / scale;
+    if (!(scale >= 1e-30f && (high - zero) * inv <= 15.4f)) return codes_exact(x, zero, scale);
+    float n[8], furthest = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float y = (x[i] - zero) * inv;
+        n[i] = (y + kRoundUp) - kRoundUp;
+        furthest = fmaxf(furthest, fabsf(y - n[i]));
+    }
+    return furthest < 0.4999f ? pack_codes(n) : codes_exact(x, zero, scale);
+}
+
+// Least and greatest of eight values, NaN if one is a NaN.
+__device__ __forceinline__ void least_greatest(const float (&f)[8], const uint4&, float& low, float& high, const float*) {
+    low = high = f[0];
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         low = fminf(low, f[i]);
         high = fmaxf(high, f[i]);
-        sum += f[i] * 0.0f;  // NaN as soon as one is an infinity or a NaN
+        sum = fmaf(f[i], 0.0f, sum);  // NaN as soon as one is an infinity or a NaN
     }
 #pragma unroll
     for (int off = 1; off < 8; off <<= 1) {
@@ -210,41 +214,171 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4TokenParams p)
         high = fmaxf(high, __shfl_xor_sync(kFullMask, high, off));
         sum += __shfl_xor_sync(kFullMask, sum, off);
     }
-    if (!go) return;
-    const bool fine = sum == 0.0f;
-    const float nan = __uint_as_float(0x7fc00000u);
-    const float zero = fine ? low + 0.0f : nan;  // -0 becomes 0
-    const float scale = fine ? scale_of(low, high, static_cast<const T*>(nullptr)) : nan;
-    unsigned word = 0;
-    if (fine && scale > 0.0f) {
-        // a scale whose reciprocal fp32 does not hold well makes every quotient an infinity or NaN here, or is far from 1e-30
-        const float inv = scale >= 1e-30f ? 1.0f / scale : nan;
+    low += sum;
+    high += sum;
+}
+template <typename T, typename T2>
+__device__ __forceinline__ void least_greatest_pairs(const uint4& raw, float& low, float& high) {
+    const T2* x = reinterpret_cast<const T2*>(&raw);
+    T2 a = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3])), b = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) word |= code_of(f[i], zero, scale, inv) << (4 * i);
+    for (int off = 1; off < 8; off <<= 1) {
+        a = __hmin2_nan(a, __shfl_xor_sync(kFullMask, a, off));
+        b = __hmax2_nan(b, __shfl_xor_sync(kFullMask, b, off));
     }
-    *reinterpret_cast<unsigned*>(piece.word) = word;
-    if (threadIdx.x % 8 == 0) write_param<T>(piece.param, scale, zero, fine);
+    low = to_float<T>(__hmin_nan(a.x, a.y));
+    high = to_float<T>(__hmax_nan(b.x, b.y));
+}
+__device__ __forceinline__ void least_greatest(const float (&)[8], const uint4& raw, float& low, float& high, const __nv_bfloat16*) {
+    least_greatest_pairs<__nv_bfloat16, __nv_bfloat162>(raw, low, high);
+}
+__device__ __forceinline__ void least_greatest(const float (&)[8], const uint4& raw, float& low, float& high, const __half*) {
+    least_greatest_pairs<__half, __half2>(raw, low, high);
+}
+
+template <typename T>
+__device__ __forceinline__ void write_param(unsigned char* p, float scale, float zero, bool fine) {
+    if (sizeof(T) == 4) {
+        const float nan = __uint_as_float(0x7fc00000u);
+        *reinterpret_cast<float2*>(p) = fine ? make_float2(scale, zero) : make_float2(nan, nan);
+    } else {
+        constexpr unsigned kNan = std::is_same<T, __half>::value ? 0x7e007e00u : 0x7fc07fc0u;
+        T two[2] = {from_float<T>(scale), from_float<T>(zero)};
+        *reinterpret_cast<unsigned*>(p) = fine ? *reinterpret_cast<const unsigned*>(two) : kNan;
+    }
+}
+
+// A token has 2 * kv_heads * D / 8 pieces of eight channels: keys of all heads, then values.  A CTA takes p.cta_tokens consecutive tokens
+// and 32 of the pieces: a lane keeps its piece, a warp takes every fourth token.  Where a token's codes go is looked up once, by one
+// thread.
+constexpr int kTokThreads = 128, kTokWarps = kTokThreads / 32, kMaxCtaTokens = 32, kBatch = 4;  // kBatch: loads of a lane that are on their way together
+
+struct Kv4Where {
+    long long dense[2];      // elements from the start of k and of v
+    unsigned char* word[2];  // the token's place in the tile of head 0, of key codes and of value codes; null: nowhere
+    unsigned char* param;
+    int t;                   // token of the tile; -1: before the row's start, 16: behind the last row
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void kv4_find(const Kv4TokenParams& p, long long i, Kv4Where& w) {
+    int row, local, position;
+    w.word[0] = w.word[1] = w.param = nullptr;
+    w.dense[0] = i * p.k_token, w.dense[1] = i * p.v_token;
+    w.t = kKv4Tile;
+    if (i >= p.total) return;
+    if (!kv4_place(p, i, row, local, position)) {
+        if (p.clear) w.t = -1;
+        return;
+    }
+    if (!p.cu) w.dense[0] = row * p.k_row + local * p.k_token, w.dense[1] = row * p.v_row + local * p.v_token;
+    w.t = position < 0 ? -1 : position % kKv4Tile;
+    if (position < 0) return;
+    int slot, inner;
+    fdivmod(position / kKv4Tile, p.cache.tiles_per_page, slot, inner);
+    const long long page = p.cache.table[(long long)row * p.cache.row_pages + slot];
+    if (page < 0 || page >= p.cache.pages) return;
+    unsigned char* tile = p.cache.pool + (page * p.cache.kv_heads * p.cache.tiles_per_page.d + inner) * (long long)p.cache.tile_bytes;
+    w.word[0] = tile + kv4_key_word<D>(w.t, 0);
+    w.word[1] = tile + kv4_value_word<D>(w.t, 0);
+    w.param = tile + 2 * kv4_code_bytes(D) + w.t * (D / kKv4Group * 2 * (int)sizeof(T));
+}
+
+// A lane's piece: what of its places does not depend on the token.
+template <typename T, int D>
+struct Kv4Piece {
+    bool there;
+    int of;  // 0 keys, 1 values
+    T* dense;
+    long long word, param;
+    const Kv4Where* where;
+
+    __device__ __forceinline__ Kv4Piece(const Kv4TokenParams& p, const Kv4Where* w) {
+        int piece = blockIdx.y * 32 + (threadIdx.x & 31);
+        const int half = p.cache.kv_heads * (D / 8);
+        there = piece < 2 * half;
+        of = piece < half ? 0 : 1;
+        piece -= of * half;
+        const int head = piece / (D / 8), c = piece % (D / 8) * 8;
+        const long long tile = (long long)head * p.cache.tiles_per_page.d * p.cache.tile_bytes;
+        dense = reinterpret_cast<T*>(of ? p.v : p.k) + head * (of ? p.v_head : p.k_head) + c;
+        word = tile + (of ? kv4_value_word<D>(0, c) - kv4_value_word<D>(0, 0) : kv4_key_word<D>(0, c));
+        param = tile + of * kv4_param_bytes(D, sizeof(T)) + c / kKv4Group * 2 * (int)sizeof(T);
+        where = w;
+    }
+    __device__ __forceinline__ T* dense_at(int token) const { return dense + where[token].dense[of]; }
+    __device__ __forceinline__ unsigned* word_at(int token) const { return reinterpret_cast<unsigned*>(where[token].word[of] + word); }
+    __device__ __forceinline__ unsigned char* param_at(int token) const { return where[token].param + param; }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTokThreads) kv4_append_kernel(const __grid_constant__ Kv4TokenParams p) {
+    __shared__ Kv4Where s_where[kMaxCtaTokens];
+    if ((int)threadIdx.x < p.cta_tokens) kv4_find<T, D>(p, (long long)blockIdx.x * p.cta_tokens + threadIdx.x, s_where[threadIdx.x]);
+    const Kv4Piece<T, D> piece(p, s_where);
+    __syncthreads();
+#pragma unroll 1
+    for (int first = threadIdx.x >> 5; first < p.cta_tokens; first += kTokWarps * kBatch) {
+        Chunk8<T> chunk[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int token = first + b * kTokWarps;
+            zero_chunk8<T>(chunk[b]);
+            if (token < p.cta_tokens && piece.there && s_where[token].param) chunk[b] = load8<T>(piece.dense_at(token), p.wide != 0);
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int token = first + b * kTokWarps;
+            if (token >= p.cta_tokens || !s_where[token].param) continue;  // all of the warp
+            float f[8], low, high;
+            unpack8(chunk[b], f);
+            least_greatest(f, raw_of(chunk[b]), low, high, static_cast<const T*>(nullptr));  // over the eight lanes of the group
+            const bool fine = fabsf(low) < INFINITY && fabsf(high) < INFINITY;
+            const float zero = low + 0.0f;  // -0 becomes 0
+            const float scale = fine ? scale_of(low, high, static_cast<const T*>(nullptr)) : 0.0f;
+            const unsigned word = scale > 0.0f ? codes_of(f, zero, high, scale, static_cast<const T*>(nullptr)) : 0u;
+            __syncwarp();
+            if (!piece.there) continue;
+            *piece.word_at(token) = word;
+            if (threadIdx.x % 8 == 0) write_param<T>(piece.param_at(token), scale, zero, fine);
+        }
+    }
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4TokenParams p) {
-    const int pieces = 2 * p.cache.kv_heads * (D / 8);
-    const long long unit = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    Kv4Piece<T, D> piece;
-    if (!kv4_piece<T, D>(p, unit, pieces, piece)) return;
-    float f[8];
-    if (piece.in_pool) {
-        const unsigned word = *reinterpret_cast<const unsigned*>(piece.word);
-        float scale, zero;
-        kv4_unpack(*reinterpret_cast<const Kv4Param<T>*>(piece.param), scale, zero);
+__global__ void __launch_bounds__(kTokThreads) kv4_read_kernel(const __grid_constant__ Kv4TokenParams p) {
+    __shared__ Kv4Where s_where[kMaxCtaTokens];
+    if ((int)threadIdx.x < p.cta_tokens) kv4_find<T, D>(p, (long long)blockIdx.x * p.cta_tokens + threadIdx.x, s_where[threadIdx.x]);
+    const Kv4Piece<T, D> piece(p, s_where);
+    __syncthreads();
+    if (!piece.there) return;
+#pragma unroll 1
+    for (int first = threadIdx.x >> 5; first < p.cta_tokens; first += kTokWarps * kBatch) {
+        unsigned word[kBatch];
+        Kv4Param<T> param[kBatch];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = fmaf((float)((word >> (4 * i)) & 15u), scale, zero);
-    } else {
-        const float fill = piece.placed ? __uint_as_float(0x7fc00000u) : 0.0f;
+        for (int b = 0; b < kBatch; ++b) {
+            const int token = first + b * kTokWarps;
+            if (token < p.cta_tokens && s_where[token].param) {
+                word[b] = *piece.word_at(token);
+                param[b] = *reinterpret_cast<const Kv4Param<T>*>(piece.param_at(token));
+            }
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = fill;
+        for (int b = 0; b < kBatch; ++b) {
+            const int token = first + b * kTokWarps;
+            if (token >= p.cta_tokens || s_where[token].t == kKv4Tile) continue;  // behind the last row's tokens: left as it was
+            Chunk8<T> out;
+            if (s_where[token].param) {
+                dequantise(word[b], param[b], out);
+            } else {
+                const T fill = from_float<T>(s_where[token].t < 0 ? 0.0f : __uint_as_float(0x7fc00000u));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(&out)[i] = fill;
+            }
+            store8(piece.dense_at(token), p.wide != 0, out);
+        }
     }
-    store8(const_cast<T*>(piece.dense), p.wide != 0, f);
 }
 
 int kv4_view(const mk36_kv4_cache* c, const char* what, Kv4View* v) {
@@ -255,6 +389,7 @@ int kv4_view(const mk36_kv4_cache* c, const char* what, Kv4View* v) {
         MK36_FAIL(MK36_ERR_INVALID_ARG, "%s: sizes must be positive", what);
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256", what);
     if (c->page_size % kKv4Tile != 0) MK36_FAIL(MK36_ERR_INVALID_ARG, "%s: page_size must be a multiple of %d", what, kKv4Tile);
+    if (c->kv_heads > 1 << 20) MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: too many heads", what);
     if (c->pages > 0x7fffffffLL) MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 pages", what);
     const long long capacity = (long long)c->row_pages * c->page_size;
     if (capacity > 0x7fffff00LL) MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: more than 2^31 - 256 tokens in a row", what);
@@ -273,12 +408,17 @@ int kv4_view(const mk36_kv4_cache* c, const char* what, Kv4View* v) {
 }
 
 template <typename T, int D>
-static int kv4_tokens_launch(const Kv4TokenParams& p, bool append, cudaStream_t s, const char* what) {
-    const long long threads = p.total * (2ll * p.cache.kv_heads * (D / 8));
-    const long long ctas = (threads + 255) / 256;
-    if (ctas > 0x7fffffffLL) MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: too many tokens for one call", what);
-    if (append) kv4_append_kernel<T, D><<<(unsigned)ctas, 256, 0, s>>>(p);
-    else kv4_read_kernel<T, D><<<(unsigned)ctas, 256, 0, s>>>(p);
+static int kv4_tokens_launch(Kv4TokenParams p, bool append, cudaStream_t s, const char* what) {
+    const DeviceInfo* info = current_device_info();
+    if (!info) return MK36_ERR_LAUNCH;
+    const long long groups = (2ll * p.cache.kv_heads * (D / 8) + 31) / 32;
+    if (groups > 65535) MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: too many heads", what);
+    // 32 tokens a CTA; fewer where that would leave SMs without work
+    p.cta_tokens = kMaxCtaTokens;
+    while (p.cta_tokens > kTokWarps && p.total * groups < p.cta_tokens * 8ll * info->sm_count) p.cta_tokens /= 2;
+    const dim3 ctas((unsigned)((p.total + p.cta_tokens - 1) / p.cta_tokens), (unsigned)groups);
+    if (append) kv4_append_kernel<T, D><<<ctas, kTokThreads, 0, s>>>(p);
+    else kv4_read_kernel<T, D><<<ctas, kTokThreads, 0, s>>>(p);
     MK36_CUDA_OK(cudaGetLastError());
     return MK36_OK;
 }
@@ -304,6 +444,7 @@ static int kv4_tokens(const mk36_kv4_cache* c, const mk36_kv4_tokens* t, bool ap
     p.v = static_cast<unsigned char*>(t->v);
     p.cu = t->cu_tokens;
     p.tokens = t->tokens;
+    p.clear = t->clear_rest;
     p.k_row = t->k_row, p.k_token = t->k_token, p.k_head = t->k_head;
     p.v_row = t->v_row, p.v_token = t->v_token, p.v_head = t->v_head;
     const int elem = kv4_elem(c->dtype);

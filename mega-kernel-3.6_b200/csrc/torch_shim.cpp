@@ -7,6 +7,7 @@
 // the reference's TORCH_CHECKs), allocates outputs, owns one workspace per device and passes raw
 // pointers and the current stream to libmk36; it contains no kernels and no arithmetic.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -605,6 +606,11 @@ std::tuple<torch::Tensor, torch::Tensor> linear_attention_decode_steps(torch::Te
 // The 4-bit paged cache.  Scratch is taken from the allocator for each call, on the current stream: calls on other streams
 // and captured graphs share none.
 // -------------------------------------------------------------------------------------------
+// These calls are a few microseconds on the GPU, so their outputs come straight from the allocator: a third of torch::empty's time.
+torch::Tensor empty_on(const torch::Tensor& like, c10::IntArrayRef sizes, torch::ScalarType type) {
+    return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+
 void check_int_table(const torch::Tensor& t, const torch::Tensor& like, const char* name, int64_t dims) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(t.device() == like.device(), name, " must be on the device of the pool");
@@ -620,12 +626,12 @@ mk36_kv4_cache kv4_cache(const torch::Tensor& pool, const torch::Tensor& pages, 
     check_int_table(pages, pool, "pages", 2);
     check_int_table(lengths, pool, "lengths", 1);
     TORCH_CHECK(lengths.size(0) == pages.size(0), "lengths must have an entry for each row of pages");
-    const torch::Tensor like = torch::empty({0}, torch::TensorOptions().dtype(dtype));
     mk36_kv4_cache c{};
-    c.dtype = dtype_code(like, "kv4 cache");
+    c.dtype = dtype == torch::kBFloat16 ? MK36_BF16 : dtype == torch::kHalf ? MK36_F16 : MK36_F32;
+    TORCH_CHECK(c.dtype != MK36_F32 || dtype == torch::kFloat, "kv4 cache: dtype ", dtype, " is not supported (bfloat16, float16, float32)");
+    const int64_t tile_bytes = head_dim * (16 + static_cast<int64_t>(c10::elementSize(dtype)));
     TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256");
-    TORCH_CHECK(pool.size(3) == head_dim * (16 + static_cast<int64_t>(like.element_size())), "pool has tiles of ", pool.size(3), " bytes, head_dim ",
-                head_dim, " in ", dtype, " takes ", head_dim * (16 + static_cast<int64_t>(like.element_size())));
+    TORCH_CHECK(pool.size(3) == tile_bytes, "pool has tiles of ", pool.size(3), " bytes, head_dim ", head_dim, " in ", dtype, " takes ", tile_bytes);
     TORCH_CHECK(pool.size(2) * 16 <= 0x7fffffff && pool.size(1) <= 0x7fffffff && pages.size(0) <= 0x7fffffff && pages.size(1) <= 0x7fffffff,
                 "pool or pages has a dimension beyond 32 bits");
     c.pool = pool.data_ptr();
@@ -680,14 +686,26 @@ void kv4_append(torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, 
     check_rc(mk36_kv4_append(&c, &t, at::cuda::getCurrentCUDAStream().stream()));
 }
 
-void kv4_read(torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, int64_t head_dim, torch::Tensor k, torch::Tensor v,
-              std::optional<torch::Tensor> cu_tokens) {
-    const mk36_kv4_cache c = kv4_cache(pool, pages, lengths, head_dim, k.scalar_type());
-    const mk36_kv4_tokens t = kv4_tokens(c, pool, k, v, cu_tokens);
+// tokens: of every row, or of all with cu_tokens; k and v are made where they are not given.
+std::tuple<torch::Tensor, torch::Tensor> kv4_read(torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, int64_t head_dim, torch::ScalarType dtype,
+                                                  int64_t tokens, std::optional<torch::Tensor> cu_tokens, std::optional<torch::Tensor> k_out,
+                                                  std::optional<torch::Tensor> v_out) {
+    const mk36_kv4_cache c = kv4_cache(pool, pages, lengths, head_dim, dtype);
+    TORCH_CHECK(tokens >= 0, "tokens must not be negative");
+    TORCH_CHECK(k_out.has_value() == v_out.has_value(), "out must be a pair of tensors");
     const c10::cuda::CUDAGuard guard(pool.device());
-    k.unsafeGetTensorImpl()->bump_version();
-    v.unsafeGetTensorImpl()->bump_version();
+    const int64_t shape[4] = {c.rows, tokens, c.kv_heads, head_dim};
+    const c10::IntArrayRef sizes = cu_tokens.has_value() ? c10::IntArrayRef(shape + 1, 3) : c10::IntArrayRef(shape, 4);
+    torch::Tensor k = k_out.has_value() ? *k_out : empty_on(pool, sizes, dtype), v = v_out.has_value() ? *v_out : empty_on(pool, sizes, dtype);
+    TORCH_CHECK(k.sizes() == sizes, "out does not have the shape of the result");
+    mk36_kv4_tokens t = kv4_tokens(c, pool, k, v, cu_tokens);
+    t.clear_rest = !k_out.has_value();
+    if (k_out.has_value()) {
+        k.unsafeGetTensorImpl()->bump_version();
+        v.unsafeGetTensorImpl()->bump_version();
+    }
     check_rc(mk36_kv4_read(&c, &t, at::cuda::getCurrentCUDAStream().stream()));
+    return {k, v};
 }
 
 torch::Tensor kv4_attention_decode(torch::Tensor q, torch::Tensor pool, torch::Tensor pages, torch::Tensor lengths, int64_t head_dim, double scale) {
@@ -702,7 +720,7 @@ torch::Tensor kv4_attention_decode(torch::Tensor q, torch::Tensor pool, torch::T
     TORCH_CHECK(q.size(-2) <= 0x7fffffff && tokens <= 0x7fffffff, "q has a dimension beyond 32 bits");
     const c10::cuda::CUDAGuard guard(pool.device());
     mk36_kv4_attention_args a{};
-    torch::Tensor out = torch::empty(q.sizes(), q.options());
+    torch::Tensor out = empty_on(pool, q.sizes(), q.scalar_type());
     a.q = q.data_ptr();
     a.out = out.data_ptr();
     a.q_row = q.stride(0);
@@ -713,7 +731,7 @@ torch::Tensor kv4_attention_decode(torch::Tensor q, torch::Tensor pool, torch::T
     a.scale = static_cast<float>(scale);
     const size_t bytes = mk36_kv4_attention_workspace_bytes(&c, &a);
     TORCH_CHECK(bytes > 0, mk36_last_error());
-    torch::Tensor scratch = torch::empty({static_cast<int64_t>(bytes)}, pool.options());
+    torch::Tensor scratch = empty_on(pool, {static_cast<int64_t>(bytes)}, torch::kUInt8);
     check_rc(mk36_kv4_attention_decode(&c, &a, scratch.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()));
     return out;
 }
@@ -730,8 +748,8 @@ PageTables kv_pages_call(const torch::Tensor& pages, const torch::Tensor& length
     TORCH_CHECK(lengths.size(0) == pages.size(0), "lengths must have an entry for each row of pages");
     TORCH_CHECK(pages.size(0) <= 0x7fffffff && pages.size(1) <= 0x7fffffff, "pages has a dimension beyond 32 bits");
     const c10::cuda::CUDAGuard guard(pages.device());
-    torch::Tensor new_pages = inplace ? pages : torch::empty_like(pages), new_lengths = inplace ? lengths : torch::empty_like(lengths);
-    torch::Tensor new_refs = inplace ? refcounts : torch::empty_like(refcounts), status = torch::empty({1}, pages.options());
+    auto made = [&](const torch::Tensor& t) { return inplace ? t : empty_on(pages, t.sizes(), torch::kInt32); };
+    torch::Tensor new_pages = made(pages), new_lengths = made(lengths), new_refs = made(refcounts), status = empty_on(pages, {1}, torch::kInt32);
     a.page_table_in = pages.data_ptr<int32_t>();
     a.lengths_in = lengths.data_ptr<int32_t>();
     a.refcounts_in = refcounts.data_ptr<int32_t>();
@@ -743,7 +761,7 @@ PageTables kv_pages_call(const torch::Tensor& pages, const torch::Tensor& length
     a.rows = static_cast<int32_t>(pages.size(0));
     a.row_pages = static_cast<int32_t>(pages.size(1));
     const size_t bytes = mk36_kv_pages_workspace_bytes(&a);
-    torch::Tensor scratch = torch::empty({static_cast<int64_t>(bytes > 0 ? bytes : 4)}, pages.options().dtype(torch::kUInt8));
+    torch::Tensor scratch = empty_on(pages, {static_cast<int64_t>(bytes > 0 ? bytes : 4)}, torch::kUInt8);
     if (inplace)
         for (const torch::Tensor* t : {&pages, &lengths, &refcounts}) t->unsafeGetTensorImpl()->bump_version();
     check_rc(call(&a, scratch.data_ptr(), bytes, at::cuda::getCurrentCUDAStream().stream()));
@@ -835,8 +853,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("decay_per_step") = py::none(), py::arg("beta_per_step") = py::none(), py::arg("inplace") = false);
     m.def("kv4_append", &kv4_append, "quantise tokens into the 4-bit paged cache", py::arg("pool"), py::arg("pages"), py::arg("lengths"),
           py::arg("head_dim"), py::arg("k"), py::arg("v"), py::arg("cu_tokens") = py::none());
-    m.def("kv4_read", &kv4_read, "read tokens of the 4-bit paged cache into k and v", py::arg("pool"), py::arg("pages"), py::arg("lengths"),
-          py::arg("head_dim"), py::arg("k"), py::arg("v"), py::arg("cu_tokens") = py::none());
+    m.def("kv4_read", &kv4_read, "read tokens of the 4-bit paged cache", py::arg("pool"), py::arg("pages"), py::arg("lengths"), py::arg("head_dim"),
+          py::arg("dtype"), py::arg("tokens"), py::arg("cu_tokens") = py::none(), py::arg("k_out") = py::none(), py::arg("v_out") = py::none());
     m.def("kv4_attention_decode", &kv4_attention_decode, "attention over the 4-bit paged cache (sm_100a)");
     m.def("kv_pages_fork", &kv_pages_fork, "rows that share another row's pages");
     m.def("kv_pages_resize", &kv_pages_resize, "take, free and copy pages for new lengths");

@@ -100,7 +100,7 @@ class Kv4Tokens(C.Structure):
     _fields_ = [
         ("k", C.c_void_p), ("v", C.c_void_p), ("cu_tokens", C.c_void_p), ("tokens", C.c_int64),
         ("k_row", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64),
-        ("v_row", C.c_int64), ("v_token", C.c_int64), ("v_head", C.c_int64),
+        ("v_row", C.c_int64), ("v_token", C.c_int64), ("v_head", C.c_int64), ("clear_rest", C.c_int32),
     ]
 
 

@@ -113,17 +113,10 @@ def kv4_read(
     ext = _native("kv4_read", cache.pool, table.pages, table.lengths)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
-    if out is None:
-        lead = (tokens,) if cu_tokens is not None else (table.pages.shape[0], tokens)
-        shape = (*lead, cache.pool.shape[1], cache.head_dim)
-        make = torch.empty if cu_tokens is None else torch.zeros
-        out = make(shape, dtype=cache.dtype, device=cache.pool.device), make(shape, dtype=cache.dtype, device=cache.pool.device)
-    k, v = out
-    _check_dtype(cache, k, v)
-    if k.shape[0 if cu_tokens is not None else 1] != tokens:
-        raise ValueError("out does not have the shape of the result")
-    ext.kv4_read(cache.pool, table.pages, table.lengths, int(cache.head_dim), k, v, cu_tokens)
-    return k, v
+    k_out, v_out = (None, None) if out is None else out
+    if out is not None:
+        _check_dtype(cache, k_out, v_out)
+    return ext.kv4_read(cache.pool, table.pages, table.lengths, int(cache.head_dim), cache.dtype, int(tokens), cu_tokens, k_out, v_out)
 
 
 def kv4_attention_decode(q: torch.Tensor, cache: Kv4Cache, table: PageTable, *, scale: Optional[float] = None) -> torch.Tensor:
