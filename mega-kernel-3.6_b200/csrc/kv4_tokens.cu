@@ -251,7 +251,7 @@ __device__ __forceinline__ void write_param(unsigned char* p, float scale, float
 // A token has 2 * kv_heads * D / 8 pieces of eight channels: keys of all heads, then values.  A CTA takes p.cta_tokens consecutive tokens
 // and 32 of the pieces: a lane keeps its piece, a warp takes every fourth token.  Where a token's codes go is looked up once, by one
 // thread.
-constexpr int kTokThreads = 128, kTokWarps = kTokThreads / 32, kMaxCtaTokens = 32, kBatch = 4;  // kBatch: loads of a lane that are on their way together
+constexpr int kTokThreads = 128, kTokWarps = kTokThreads / 32, kMaxCtaTokens = 32, kBatch = 2;  // kBatch: loads of a lane that are on their way together
 
 struct Kv4Where {
     long long dense[2];      // elements from the start of k and of v

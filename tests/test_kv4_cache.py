@@ -764,3 +764,43 @@ def test_calls_on_the_gpu_refuse_wrong_arguments(cuda_device):
         with pytest.raises((RuntimeError, ValueError), match=text):
             wrong()
     s.same_pool()
+
+
+@pytest.mark.gpu
+def test_more_pages_than_a_plan_ranks_at_once(cuda_device):
+    """Pages by the ten thousand: ranks carry over from one segment of 32768 to the next."""
+    total, rows, width = 70_001, 300, 260
+    cache = mk.Kv4Cache(torch.zeros(total, 1, 1, oracle.tile_bytes(64, torch.float16), dtype=torch.uint8, device=cuda_device), 64, torch.float16)
+    cache.pool[:, 0, 0, :4] = torch.arange(total, dtype=torch.int32, device=cuda_device).view(torch.uint8).view(total, 4)  # each page knows its number
+    rng = random.Random(4)
+    ids, at = rng.sample(range(total), total), 0
+    table, lengths, refs = [], [], [0] * total
+    for r in range(rows):
+        n = rng.randrange(0, width)
+        lengths.append(16 * n - rng.randrange(0, 16) if n else 0)
+        table.append(ids[at : at + n] + [-1] * (width - n))
+        for p in ids[at : at + n]:
+            refs[p] = 1
+        at += n
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)
+    gpu = mk.PageTable(on(table), on(lengths), on(refs))
+    pool = cache.pool.cpu().numpy().copy()
+    after = [rng.choice([0, n, min(16 * width, n + 1), rng.randrange(0, 16 * width)]) for n in lengths]
+    *state, status = oracle.resize(pool, table, lengths, refs, after)
+    gpu, got = mk.kv_pages_resize(cache, gpu, on(after))
+    assert got.item() == status == 0 and _lists(gpu) == tuple(state)
+    *state, n = oracle.compact(pool, *state)
+    gpu, got = mk.kv_pages_compact(cache, gpu)
+    assert got.item() == n and _lists(gpu) == tuple(state) and np.array_equal(cache.pool.cpu().numpy(), pool)
+    *state, status = oracle.resize(pool, *state, [16 * width] * rows)
+    gpu, got = mk.kv_pages_resize(cache, gpu, on([16 * width] * rows))
+    assert got.item() == status > 0 and _lists(gpu) == tuple(state)
+    # more than one segment in use, and holes in each
+    for after in ([16 * 200] * rows, [16 * (240 if r % 2 else 100) for r in range(rows)], [16 * 225] * rows, [16 * (250 if r % 3 else 150) for r in range(rows)]):
+        *state, status = oracle.resize(pool, *state, after)
+        gpu, got = mk.kv_pages_resize(cache, gpu, on(after))
+        assert got.item() == status and _lists(gpu) == tuple(state)
+    assert status == 0
+    *state, n = oracle.compact(pool, *state)
+    gpu, got = mk.kv_pages_compact(cache, gpu)
+    assert got.item() == n > 32768 and _lists(gpu) == tuple(state) and np.array_equal(cache.pool.cpu().numpy(), pool)
