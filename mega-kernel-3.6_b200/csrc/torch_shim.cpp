@@ -748,8 +748,19 @@ PageTables kv_pages_call(const torch::Tensor& pages, const torch::Tensor& length
     TORCH_CHECK(lengths.size(0) == pages.size(0), "lengths must have an entry for each row of pages");
     TORCH_CHECK(pages.size(0) <= 0x7fffffff && pages.size(1) <= 0x7fffffff, "pages has a dimension beyond 32 bits");
     const c10::cuda::CUDAGuard guard(pages.device());
-    auto made = [&](const torch::Tensor& t) { return inplace ? t : empty_on(pages, t.sizes(), torch::kInt32); };
-    torch::Tensor new_pages = made(pages), new_lengths = made(lengths), new_refs = made(refcounts), status = empty_on(pages, {1}, torch::kInt32);
+    // the new tables and the status share one allocation
+    auto round_up = [](int64_t n) { return (n + 63) / 64 * 64; };
+    const int64_t n_pages = inplace ? 0 : round_up(pages.numel()), n_lengths = inplace ? 0 : round_up(lengths.numel()),
+                  n_refs = inplace ? 0 : round_up(refcounts.numel());
+    const torch::Tensor made = empty_on(pages, {n_pages + n_lengths + n_refs + 1}, torch::kInt32);
+    auto part = [&](c10::IntArrayRef sizes, int64_t offset) {
+        auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(made.storage()), made.key_set(), made.dtype());
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+        t.unsafeGetTensorImpl()->set_storage_offset(offset);
+        return t;
+    };
+    torch::Tensor new_pages = inplace ? pages : part(pages.sizes(), 0), new_lengths = inplace ? lengths : part(lengths.sizes(), n_pages);
+    torch::Tensor new_refs = inplace ? refcounts : part(refcounts.sizes(), n_pages + n_lengths), status = part({1}, n_pages + n_lengths + n_refs);
     a.page_table_in = pages.data_ptr<int32_t>();
     a.lengths_in = lengths.data_ptr<int32_t>();
     a.refcounts_in = refcounts.data_ptr<int32_t>();
