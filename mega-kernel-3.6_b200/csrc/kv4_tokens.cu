@@ -59,10 +59,6 @@ __device__ __forceinline__ Chunk8<T> load8(const T* p, bool wide) {
     for (int i = 0; i < 8; ++i) x[i] = p[i];
     return c;
 }
-__device__ __forceinline__ const uint4& raw_of(const Chunk8<float>& c) { return c.lo; }
-template <typename T>
-__device__ __forceinline__ const uint4& raw_of(const Chunk8<T>& c) { return c.raw; }
-
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool wide, const Chunk8<T>& c) {
     if (wide) {
@@ -154,11 +150,7 @@ __device__ __forceinline__ unsigned pack_codes(const float (&n)[8]) {
 // bits at most; x - zero has 24 and is off by e at most half its last place; half the scale is a multiple of that place.)
 // Values half way between two codes are common, one in some hundred of bf16: about every second warp has one.
 template <typename T>
-__device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, float high, float scale, const T*) {
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
-    // scales of a few units of the smallest number, whose quotients may be far beyond 15, and what the reciprocal does not hold
-    if (!(scale >= 1e-30f && (high - zero) * inv <= 15.4f)) return codes_exact(x, zero, scale);
+__device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, float scale, float inv, const T*) {
     const float half = 0.5f * scale;
     float n[8], r[8];
     bool border = false;
@@ -185,9 +177,7 @@ __device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, fl
 
 // Codes of fp32 values: neither the difference nor the product is exact, so near a border fp64 decides.  The quotient is off by less than
 // 2e-5: difference, product and reciprocal by 2^-23 or less each.
-__device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, float high, float scale, const float*) {
-    const float inv = 1.0f / scale;
-    if (!(scale >= 1e-30f && (high - zero) * inv <= 15.4f)) return codes_exact(x, zero, scale);
+__device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, float scale, float inv, const float*) {
     float n[8], furthest = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -198,18 +188,32 @@ __device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, fl
     return furthest < 0.4999f ? pack_codes(n) : codes_exact(x, zero, scale);
 }
 
-// Least and greatest of eight values, NaN if one is a NaN.
-__device__ __forceinline__ void least_greatest(const float (&f)[8], const uint4&, float& low, float& high, const float*) {
+// Codes of a group's part, two words of eight: what both kinds share.
+template <typename T>
+__device__ __forceinline__ uint2 two_words(const float (&x)[16], float zero, float high, float scale) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    if (sizeof(T) == 4) inv = 1.0f / scale;
+    const float(&first)[8] = *reinterpret_cast<const float(*)[8]>(&x[0]);
+    const float(&second)[8] = *reinterpret_cast<const float(*)[8]>(&x[8]);
+    if (!(scale > 0.0f)) return make_uint2(0u, 0u);
+    // scales of a few units of the smallest number, whose quotients may be far beyond 15, and what the reciprocal does not hold
+    if (!(scale >= 1e-30f && (high - zero) * inv <= 15.4f)) return make_uint2(codes_exact(first, zero, scale), codes_exact(second, zero, scale));
+    return make_uint2(codes_of(first, zero, scale, inv, static_cast<const T*>(nullptr)), codes_of(second, zero, scale, inv, static_cast<const T*>(nullptr)));
+}
+
+// Least and greatest of the 64 values of four lanes, 16 of each; NaN if one is a NaN.
+__device__ __forceinline__ void least_greatest(const float (&f)[16], const Chunk8<float> (&)[2], float& low, float& high) {
     low = high = f[0];
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
         low = fminf(low, f[i]);
         high = fmaxf(high, f[i]);
         sum = fmaf(f[i], 0.0f, sum);  // NaN as soon as one is an infinity or a NaN
     }
 #pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
+    for (int off = 1; off < 4; off <<= 1) {
         low = fminf(low, __shfl_xor_sync(kFullMask, low, off));
         high = fmaxf(high, __shfl_xor_sync(kFullMask, high, off));
         sum += __shfl_xor_sync(kFullMask, sum, off);
@@ -217,23 +221,24 @@ __device__ __forceinline__ void least_greatest(const float (&f)[8], const uint4&
     low += sum;
     high += sum;
 }
-template <typename T, typename T2>
-__device__ __forceinline__ void least_greatest_pairs(const uint4& raw, float& low, float& high) {
-    const T2* x = reinterpret_cast<const T2*>(&raw);
-    T2 a = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3])), b = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+template <typename T2, typename T>
+__device__ __forceinline__ void least_greatest_pairs(const Chunk8<T> (&c)[2], float& low, float& high) {
+    const T2 *x = reinterpret_cast<const T2*>(&c[0]), *y = reinterpret_cast<const T2*>(&c[1]);
+    T2 a = __hmin2_nan(__hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3])), __hmin2_nan(__hmin2_nan(y[0], y[1]), __hmin2_nan(y[2], y[3])));
+    const T2 b = __hmax2_nan(__hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3])), __hmax2_nan(__hmax2_nan(y[0], y[1]), __hmax2_nan(y[2], y[3])));
+    // the least and the greatest, less its sign, travel as one pair
+    a.x = __hmin_nan(a.x, a.y);
+    a.y = __hneg(__hmax_nan(b.x, b.y));
 #pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
-        a = __hmin2_nan(a, __shfl_xor_sync(kFullMask, a, off));
-        b = __hmax2_nan(b, __shfl_xor_sync(kFullMask, b, off));
-    }
-    low = to_float<T>(__hmin_nan(a.x, a.y));
-    high = to_float<T>(__hmax_nan(b.x, b.y));
+    for (int off = 1; off < 4; off <<= 1) a = __hmin2_nan(a, __shfl_xor_sync(kFullMask, a, off));
+    low = to_float<T>(a.x);
+    high = -to_float<T>(a.y);
 }
-__device__ __forceinline__ void least_greatest(const float (&)[8], const uint4& raw, float& low, float& high, const __nv_bfloat16*) {
-    least_greatest_pairs<__nv_bfloat16, __nv_bfloat162>(raw, low, high);
+__device__ __forceinline__ void least_greatest(const float (&)[16], const Chunk8<__nv_bfloat16> (&c)[2], float& low, float& high) {
+    least_greatest_pairs<__nv_bfloat162>(c, low, high);
 }
-__device__ __forceinline__ void least_greatest(const float (&)[8], const uint4& raw, float& low, float& high, const __half*) {
-    least_greatest_pairs<__half, __half2>(raw, low, high);
+__device__ __forceinline__ void least_greatest(const float (&)[16], const Chunk8<__half> (&c)[2], float& low, float& high) {
+    least_greatest_pairs<__half2>(c, low, high);
 }
 
 template <typename T>
@@ -248,7 +253,7 @@ __device__ __forceinline__ void write_param(unsigned char* p, float scale, float
     }
 }
 
-// A token has 2 * kv_heads * D / 8 pieces of eight channels: keys of all heads, then values.  A CTA takes p.cta_tokens consecutive tokens
+// A token has pieces of 8 channels (read) or 16 (append): keys of all heads, then values.  A CTA takes p.cta_tokens consecutive tokens
 // and 32 of the pieces: a lane keeps its piece, a warp takes every fourth token.  Where a token's codes go is looked up once, by one
 // thread.
 constexpr int kTokThreads = 128, kTokWarps = kTokThreads / 32, kMaxCtaTokens = 32, kBatch = 2;  // kBatch: loads of a lane that are on their way together
@@ -285,7 +290,7 @@ __device__ __forceinline__ void kv4_find(const Kv4TokenParams& p, long long i, K
 }
 
 // A lane's piece: what of its places does not depend on the token.
-template <typename T, int D>
+template <typename T, int D, int kChannels>
 struct Kv4Piece {
     bool there;
     int of;  // 0 keys, 1 values
@@ -295,11 +300,11 @@ struct Kv4Piece {
 
     __device__ __forceinline__ Kv4Piece(const Kv4TokenParams& p, const Kv4Where* w) {
         int piece = blockIdx.y * 32 + (threadIdx.x & 31);
-        const int half = p.cache.kv_heads * (D / 8);
+        const int half = p.cache.kv_heads * (D / kChannels);
         there = piece < 2 * half;
         of = piece < half ? 0 : 1;
         piece -= of * half;
-        const int head = piece / (D / 8), c = piece % (D / 8) * 8;
+        const int head = piece / (D / kChannels), c = piece % (D / kChannels) * kChannels;
         const long long tile = (long long)head * p.cache.tiles_per_page.d * p.cache.tile_bytes;
         dense = reinterpret_cast<T*>(of ? p.v : p.k) + head * (of ? p.v_head : p.k_head) + c;
         word = tile + (of ? kv4_value_word<D>(0, c) - kv4_value_word<D>(0, 0) : kv4_key_word<D>(0, c));
@@ -315,32 +320,43 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kTokThreads) kv4_append_kernel(const __grid_constant__ Kv4TokenParams p) {
     __shared__ Kv4Where s_where[kMaxCtaTokens];
     if ((int)threadIdx.x < p.cta_tokens) kv4_find<T, D>(p, (long long)blockIdx.x * p.cta_tokens + threadIdx.x, s_where[threadIdx.x]);
-    const Kv4Piece<T, D> piece(p, s_where);
+    const Kv4Piece<T, D, 16> piece(p, s_where);  // four lanes have a group
     __syncthreads();
 #pragma unroll 1
     for (int first = threadIdx.x >> 5; first < p.cta_tokens; first += kTokWarps * kBatch) {
-        Chunk8<T> chunk[kBatch];
+        Chunk8<T> chunk[kBatch][2];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const int token = first + b * kTokWarps;
-            zero_chunk8<T>(chunk[b]);
-            if (token < p.cta_tokens && piece.there && s_where[token].param) chunk[b] = load8<T>(piece.dense_at(token), p.wide != 0);
+            zero_chunk8<T>(chunk[b][0]);
+            zero_chunk8<T>(chunk[b][1]);
+            if (token < p.cta_tokens && piece.there && s_where[token].param) {
+                const T* src = piece.dense_at(token);
+                chunk[b][0] = load8<T>(src, p.wide != 0);
+                chunk[b][1] = load8<T>(src + 8, p.wide != 0);
+            }
         }
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const int token = first + b * kTokWarps;
             if (token >= p.cta_tokens || !s_where[token].param) continue;  // all of the warp
-            float f[8], low, high;
-            unpack8(chunk[b], f);
-            least_greatest(f, raw_of(chunk[b]), low, high, static_cast<const T*>(nullptr));  // over the eight lanes of the group
+            float f[16], low, high;
+            unpack8(chunk[b][0], *reinterpret_cast<float(*)[8]>(&f[0]));
+            unpack8(chunk[b][1], *reinterpret_cast<float(*)[8]>(&f[8]));
+            least_greatest(f, chunk[b], low, high);
             const bool fine = fabsf(low) < INFINITY && fabsf(high) < INFINITY;
             const float zero = low + 0.0f;  // -0 becomes 0
             const float scale = fine ? scale_of(low, high, static_cast<const T*>(nullptr)) : 0.0f;
-            const unsigned word = scale > 0.0f ? codes_of(f, zero, high, scale, static_cast<const T*>(nullptr)) : 0u;
+            const uint2 words = two_words<T>(f, zero, high, scale);
             __syncwarp();
             if (!piece.there) continue;
-            *piece.word_at(token) = word;
-            if (threadIdx.x % 8 == 0) write_param<T>(piece.param_at(token), scale, zero, fine);
+            if (piece.of == 0) {
+                *reinterpret_cast<uint2*>(piece.word_at(token)) = words;
+            } else {
+                piece.word_at(token)[0] = words.x;
+                piece.word_at(token)[D / 16] = words.y;  // four units on: the next eight channels' lane
+            }
+            if (threadIdx.x % 4 == 0) write_param<T>(piece.param_at(token), scale, zero, fine);
         }
     }
 }
@@ -349,7 +365,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kTokThreads) kv4_read_kernel(const __grid_constant__ Kv4TokenParams p) {
     __shared__ Kv4Where s_where[kMaxCtaTokens];
     if ((int)threadIdx.x < p.cta_tokens) kv4_find<T, D>(p, (long long)blockIdx.x * p.cta_tokens + threadIdx.x, s_where[threadIdx.x]);
-    const Kv4Piece<T, D> piece(p, s_where);
+    const Kv4Piece<T, D, 8> piece(p, s_where);
     __syncthreads();
     if (!piece.there) return;
 #pragma unroll 1
@@ -411,7 +427,7 @@ template <typename T, int D>
 static int kv4_tokens_launch(Kv4TokenParams p, bool append, cudaStream_t s, const char* what) {
     const DeviceInfo* info = current_device_info();
     if (!info) return MK36_ERR_LAUNCH;
-    const long long groups = (2ll * p.cache.kv_heads * (D / 8) + 31) / 32;
+    const long long groups = (2ll * p.cache.kv_heads * (D / (append ? 16 : 8)) + 31) / 32;
     if (groups > 65535) MK36_FAIL(MK36_ERR_UNSUPPORTED, "%s: too many heads", what);
     // 32 tokens a CTA; fewer where that would leave SMs without work
     p.cta_tokens = kMaxCtaTokens;
