@@ -48,8 +48,9 @@ struct Kv4AttnParams {
 // Partial results: per (CTA, first or last segment) and column the sums, then maximum (of scores in units of log 2) and sum of weights.
 __host__ __device__ constexpr int ka_slot_floats(int d) { return 8 * (d + 4); }
 
-// What their registers leave room for.
-__host__ __device__ constexpr int ka_ctas_per_sm(bool fp32, int d) { return (fp32 ? 2 : 3) + (d == 64 ? 1 : 0); }
+// As many as their registers leave room for without spills (heads of 128 in three: 74 us where four take 69; heads of 256 in four, which
+// spill: 110 us where three take 78).
+__host__ __device__ constexpr int ka_ctas_per_sm(bool fp32, int d) { return fp32 ? (d == 64 ? 3 : 2) : (d == 256 ? 3 : 4); }
 
 
 template <typename T, int D>
