@@ -2,21 +2,29 @@
 //
 // Mathematics.  A key entry stands for z + n s with a code n of 4 bits and s, z of its group of 64 channels, a value entry likewise:
 //     score_t = sum_groups s_tg (q_g . n_tg) + z_tg sum(q_g)          out_c = sum_t (p_t s'_tg) n'_tc + sum_t p_t z'_tg
-// so scales and zero points never touch an element: keys get theirs on the products of a group, values on the weights.  What is left
-// per element is to turn codes into operands, and there f16 helps: the bits 0x000n are the subnormal n 2^-24, 0x00n0 is n 2^-20, so
-// a 32-bit word of eight codes becomes four operand registers with four masks and one shift (five instructions for eight codes).  The
-// factor 16 of every second register goes into q (keys) or into the result (values).
-//   q is scaled by a power of two so that its largest channel is in [2^14, 2^15), exact for bf16 and for f16.  Weights times scales
-// are divided by the power of two of the largest scale met so far, so that f16 holds them whatever the size of the values; they are held
-// in two halves (hi + lo, 22 bits), because what the codes stand for has a zero point: the error of a rounded weight would be
-// multiplied by a code of 0 .. 15 where the value itself may be near zero.
+// so scales and zero points never touch an element: keys get theirs on the products of a group, values on the weights, and the two sums
+// with zero points are small matrix products of their own (tokens x groups by groups x columns; groups x tokens by tokens x columns).
+// What is left per element is to turn codes into operands, and there f16 helps: the bits 0x000n are the subnormal n 2^-24, 0x00n0 is
+// n 2^-20, so a 32-bit word of eight codes becomes four operand registers with four masks and one shift.  The factor 16 of every
+// second register goes into q (keys) or into the result (values).
+//   * q is scaled by a power of two so that its largest channel is in [2^14, 2^15): exact for bf16 and f16 values.
+//   * Weights times scales are kept in units of the largest scale's power of two so far, so that f16 holds them whatever the size of the
+//     values, and in two halves (hi + lo, 22 bits): a rounded weight's error would be multiplied by a code of 0 .. 15 where the value
+//     itself, with its zero point, may be near zero.  (One half: 6 us of 78 less at 48 long rows, and an error of 2^-11 of the codes' size.)
+//   * fp32 splits its queries the same way, takes codes less 8, and adds up short chains of products in fp32 (its error against 64 bits
+//     is 2e-7 to 5e-7 of the output, that of sums in fp32 throughout 2e-7 to 9e-7).
 //
-// Work.  Four warps a CTA, two CTAs an SM.  A warp takes a tile (16 tokens of a KV head) on its own: scores as MMAs of 16 tokens x 16
-// channels by 8 columns (the query heads and tokens that share the KV head), a transposition of the 16 x 8 scores inside the warp,
-// running maximum and sum, values as MMAs of 16 channels x 16 tokens.  Tiles come through a ring of the warp's own, one bulk copy
-// each (a tile is contiguous), so that nothing but the end of a segment needs the other warps.  All tiles of all rows and heads form one line
-// that is cut into as many equal pieces as there are CTAs; a piece that ends inside a row leaves a partial result, and a second launch
-// joins those.
+// Work.  Four warps a CTA, three CTAs an SM (heads of 256).  A warp takes a tile (16 tokens of a KV head) on its own: scores as MMAs of 16
+// tokens x 16 channels by 8 columns (the query heads and tokens that share the KV head), a transposition of the 16 x 8 scores inside
+// the warp, weights relative to a maximum that moves only when it has to, values as MMAs of 16 channels x 16 tokens.  Tiles come through a
+// ring of the warp's own, one bulk copy each (a tile is contiguous), so that nothing but the end of a segment needs the other warps.  All
+// tiles of all rows and heads form one line that is cut into as many equal pieces as there are CTAs; a piece that ends inside a row
+// leaves a partial result, and a second launch, set up while the first still runs, joins those.
+//
+// What bounds it.  Short rows: latency, 9.6 us for one row of 700 tokens.  Many long rows: not memory (tiles that all lie in L2 take 97 % of
+// the time) but the SMs: 626 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
+// of 8 cycles; issue slots, that pipe, the tensor cores and shared memory are each 40 to 60 % busy, with three warps a scheduler.  48 rows
+// of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78 us, 3.5 TB/s; 24 / 4 heads, three tokens, 12 rows: 42.8 us.
 #include <math.h>
 
 #include <type_traits>
@@ -29,7 +37,7 @@ namespace mk36 {
 
 constexpr int kKaWarps = 4;
 constexpr int kKaThreads = kKaWarps * 32;
-constexpr int kKaMinTiles = 8;     // fewest tiles of a piece: two a warp
+constexpr int kKaMinTiles = kKaWarps;  // fewest tiles of a piece: one a warp (one row of 700 tokens: 9.6 us; two a warp 12.6, four 14.8)
 
 struct Kv4AttnParams {
     Kv4View cache;

@@ -2,13 +2,13 @@
 // page before it is written), and making the pool dense.
 //
 // Every operator is two launches.  A plan kernel of one CTA checks the request, counts, and ranks with prefix sums, so that the outcome
-// does not depend on the order of threads (the only atomics are additions of whole numbers); it writes what is to be done to scratch
-// and not to the tables (but for a copy of the reference counts that fork adds to).  An apply kernel over the whole GPU then writes the tables and moves the pages, or, where the plan
-// found the request impossible, hands the tables on as they were.  Because everything that an apply thread reads of another
-// thread's entry lies in scratch, tables may be changed where they lie.
+// does not depend on the order of threads (the only atomics are additions of whole numbers); it writes what is to be done to scratch and
+// not to the tables (but for a copy of the reference counts that fork adds to).  An apply kernel over the whole GPU then writes the
+// tables and moves the pages, or, where the plan found the request impossible, hands the tables on as they were.  Because everything
+// that an apply thread reads of another thread's entry lies in scratch, tables may be changed where they lie.
 //
-// What bounds them: the copies run at memory speed; the rest is latency of two dependent launches and of a few passes of one CTA
-// over the reference counts (4 bytes a page).
+// What bounds them: the copies run at memory speed (3400 pages of 36 KB: 250 MB there and back in 38 us, 6.6 TB/s); the rest is latency
+// of two dependent launches and of the plan's chain of loads (fork 3 us, resize 6 to 10 us for 200 rows and 8200 pages, compact 3 to 9 us).
 #include "mk36_kv4.cuh"
 
 namespace mk36 {
