@@ -106,18 +106,23 @@ __device__ __forceinline__ bool ranked(const PageBits& b, int i, int& before) {
 
 __device__ __forceinline__ int pages_of(int length, int page_size) { return length > 0 ? (length - 1) / page_size + 1 : 0; }
 
+// A plan does not write the tables that it is given, so it may read them with __ldg: such loads need not wait for the stores before them.
+
 // ---- fork ---------------------------------------------------------------------------------------------------------------
 
 __global__ void __launch_bounds__(kPlanThreads) kv_fork_plan_kernel(const __grid_constant__ PagesParams p) {
     __shared__ int s_bad;
     let_apply_start();
     if (threadIdx.x == 0) s_bad = 0;
+#pragma unroll 4
     for (int r = threadIdx.x; r < p.rows; r += kPlanThreads) {
         p.source[r] = -1;  // parent of the row, if it becomes a child
-        p.old_len[r] = p.lengths_in[r];
+        p.old_len[r] = __ldg(&p.lengths_in[r]);
     }
-    if (p.refs_out != p.refs_in)
-        for (int i = threadIdx.x; i < p.pages; i += kPlanThreads) p.refs_out[i] = p.refs_in[i];
+    if (p.refs_out != p.refs_in) {
+#pragma unroll 8
+        for (int i = threadIdx.x; i < p.pages; i += kPlanThreads) p.refs_out[i] = __ldg(&p.refs_in[i]);
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < p.count; i += kPlanThreads) {
         const int parent = p.parents[i], child = p.children[i];
@@ -158,14 +163,15 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_plan_kernel(const __gr
     const int capacity = p.row_pages * p.page_size;
     let_apply_start();
     if (threadIdx.x == 0) s_bad = 0;
-    for (int i = threadIdx.x; i < p.pages; i += kPlanThreads) p.refs[i] = p.refs_in[i];
+#pragma unroll 8
+    for (int i = threadIdx.x; i < p.pages; i += kPlanThreads) p.refs[i] = __ldg(&p.refs_in[i]);
     for (int base = 0; base < p.rows; base += kPlanThreads) {
         // the rows that shrink are listed (in any order: what follows are sums), then a warp for each gives back what lies behind its new end
         if (threadIdx.x == 0) s_rows = 0;
         __syncthreads();
         const int row = base + threadIdx.x;
         if (row < p.rows) {
-            const int a = p.lengths_in[row], b = p.new_lengths[row];
+            const int a = __ldg(&p.lengths_in[row]), b = __ldg(&p.new_lengths[row]);
             p.old_len[row] = a;
             p.new_len[row] = b;
             if (a < 0 || b < 0 || a > capacity || b > capacity) s_bad = 1;
@@ -295,15 +301,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv_compact_plan_kernel(const __g
             ranked(s_bits, n - first, rank);
             front = before + rank;
         }
+#pragma unroll 4
         for (int i = threadIdx.x; i < end; i += kPlanThreads) {
-            const int page = first + i;
+            const int page = first + i, refs = __ldg(&p.refs_in[page]);
             int rank;
             if (ranked(s_bits, i, rank)) {
                 if (page >= n) p.other[before + rank - front] = page;
             } else if (page < n) {
                 p.list[page - before - rank] = page;
             }
-            p.refs[page] = page < n ? p.refs_in[page] : 0;
+            p.refs[page] = page < n ? refs : 0;
         }
         before += used_here;
         __syncthreads();

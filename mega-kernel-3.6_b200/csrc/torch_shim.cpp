@@ -611,6 +611,14 @@ torch::Tensor empty_on(const torch::Tensor& like, c10::IntArrayRef sizes, torch:
     return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
+// A dense tensor over a part of another one's memory.
+torch::Tensor part_of(const torch::Tensor& whole, c10::IntArrayRef sizes, int64_t offset) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    return t;
+}
+
 void check_int_table(const torch::Tensor& t, const torch::Tensor& like, const char* name, int64_t dims) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(t.device() == like.device(), name, " must be on the device of the pool");
@@ -696,7 +704,14 @@ std::tuple<torch::Tensor, torch::Tensor> kv4_read(torch::Tensor pool, torch::Ten
     const c10::cuda::CUDAGuard guard(pool.device());
     const int64_t shape[4] = {c.rows, tokens, c.kv_heads, head_dim};
     const c10::IntArrayRef sizes = cu_tokens.has_value() ? c10::IntArrayRef(shape + 1, 3) : c10::IntArrayRef(shape, 4);
-    torch::Tensor k = k_out.has_value() ? *k_out : empty_on(pool, sizes, dtype), v = v_out.has_value() ? *v_out : empty_on(pool, sizes, dtype);
+    torch::Tensor k, v;
+    if (k_out.has_value()) {
+        k = *k_out, v = *v_out;
+    } else {  // both in one allocation
+        const int64_t n = c10::multiply_integers(sizes);
+        const torch::Tensor both = empty_on(pool, {2 * n}, dtype);
+        k = part_of(both, sizes, 0), v = part_of(both, sizes, n);
+    }
     TORCH_CHECK(k.sizes() == sizes, "out does not have the shape of the result");
     mk36_kv4_tokens t = kv4_tokens(c, pool, k, v, cu_tokens);
     t.clear_rest = !k_out.has_value();
@@ -753,14 +768,9 @@ PageTables kv_pages_call(const torch::Tensor& pages, const torch::Tensor& length
     const int64_t n_pages = inplace ? 0 : round_up(pages.numel()), n_lengths = inplace ? 0 : round_up(lengths.numel()),
                   n_refs = inplace ? 0 : round_up(refcounts.numel());
     const torch::Tensor made = empty_on(pages, {n_pages + n_lengths + n_refs + 1}, torch::kInt32);
-    auto part = [&](c10::IntArrayRef sizes, int64_t offset) {
-        auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(made.storage()), made.key_set(), made.dtype());
-        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-        t.unsafeGetTensorImpl()->set_storage_offset(offset);
-        return t;
-    };
-    torch::Tensor new_pages = inplace ? pages : part(pages.sizes(), 0), new_lengths = inplace ? lengths : part(lengths.sizes(), n_pages);
-    torch::Tensor new_refs = inplace ? refcounts : part(refcounts.sizes(), n_pages + n_lengths), status = part({1}, n_pages + n_lengths + n_refs);
+    torch::Tensor new_pages = inplace ? pages : part_of(made, pages.sizes(), 0), new_lengths = inplace ? lengths : part_of(made, lengths.sizes(), n_pages);
+    torch::Tensor new_refs = inplace ? refcounts : part_of(made, refcounts.sizes(), n_pages + n_lengths);
+    torch::Tensor status = part_of(made, {1}, n_pages + n_lengths + n_refs);
     a.page_table_in = pages.data_ptr<int32_t>();
     a.lengths_in = lengths.data_ptr<int32_t>();
     a.refcounts_in = refcounts.data_ptr<int32_t>();
