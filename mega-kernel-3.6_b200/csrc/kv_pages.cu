@@ -7,8 +7,8 @@
 // tables and moves the pages, or, where the plan found the request impossible, hands the tables on as they were.  Because everything
 // that an apply thread reads of another thread's entry lies in scratch, tables may be changed where they lie.
 //
-// What bounds them: the copies run at memory speed (3400 pages of 36 KB: 250 MB there and back in 38 us, 6.6 TB/s); the rest is latency
-// of two dependent launches and of the plan's chain of loads (fork 3 us, resize 6 to 10 us for 200 rows and 8200 pages, compact 3 to 9 us).
+// What bounds them: the copies run at memory speed (3000 pages of 36 KB: 221 MB there and back in 36 us, 6.1 TB/s); the rest is latency
+// of two dependent launches and of the plan's chain of loads (fork 3 us, resize 6 to 10 us, 200 rows and 8500 pages the latter, compact 3 to 9 us).
 #include "mk36_kv4.cuh"
 
 namespace mk36 {
