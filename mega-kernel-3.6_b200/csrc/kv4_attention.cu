@@ -46,7 +46,7 @@ struct Kv4AttnParams {
     float* partial;
     long long q_row, q_token, q_head;
     int query_heads, tokens, group, columns;  // group: query heads of a KV head; columns: group * tokens
-    int blocks;                               // pieces of the columns, 8 or 16 each
+    int blocks;                               // of eight columns
     int streams;                              // kv_heads * blocks: passes over a row
     int ctas, wide_q, join_parts, join_threads;
     float scale;
@@ -59,7 +59,6 @@ __host__ __device__ constexpr int ka_slot_floats(int d) { return 8 * (d + 4); }
 // As many as their registers leave room for without spills (heads of 128 in three: 74 us where four take 69; heads of 256 in four, which
 // spill: 110 us where three take 78).
 __host__ __device__ constexpr int ka_ctas_per_sm(bool fp32, int d) { return fp32 ? (d == 64 ? 3 : 2) : (d == 256 ? 3 : 4); }
-
 
 template <typename T, int D>
 struct KaConfig {
@@ -231,7 +230,7 @@ __device__ __forceinline__ void load_params(const unsigned char* p, float (&s)[G
             s[i] = __uint_as_float(w[(2 * i) % (G * (int)sizeof(T) / 2)]);
             z[i] = __uint_as_float(w[(2 * i + 1) % (G * (int)sizeof(T) / 2)]);
         } else {
-            Kv4Param<typename std::conditional<sizeof(T) == 4, __half, T>::type> one{w[i]};
+            Kv4Param<typename std::conditional<sizeof(T) == 4, __half, T>::type> one{w[i]};  // fp32 does not come here
             kv4_unpack(one, s[i], z[i]);
         }
     }
@@ -257,22 +256,21 @@ __device__ __forceinline__ void ka_advance(const Kv4AttnParams& p, KaCursor& c, 
     }
 }
 
-// All CTAs cut the line alike: tiles of all rows, and the piece length.  Every thread calls it; s: 32 words.
-template <int kThreads>
-__device__ __forceinline__ int ka_line(const Kv4AttnParams& p, int rows, int* s) {
-    int mine = 0;  // the whole line is below 2^31 tiles, which the host sees to
-    for (int r = threadIdx.x; r < rows; r += kThreads) mine += ka_tiles(p.cache, r);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(kFullMask, mine, off);
+// Tiles of the whole line, below 2^31 as the host sees to.  Every thread of the attention kernel calls it; s: a word for each warp.
+__device__ __forceinline__ int ka_line(const Kv4AttnParams& p, int* s) {
+    int mine = 0;
+    for (int r = threadIdx.x; r < p.cache.rows; r += kKaThreads) mine += ka_tiles(p.cache, r);
+    mine = __reduce_add_sync(kFullMask, mine);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = mine;
     __syncthreads();
     int sum = 0;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) sum += s[w];
+    for (int w = 0; w < kKaWarps; ++w) sum += s[w];
     return sum * p.streams;
 }
 
+// All CTAs, and the join, cut the line alike.
 __device__ __forceinline__ int ka_piece(int total, int ctas) {
     return max(kKaMinTiles, (int)(((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas));
 }
@@ -306,7 +304,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
     {
         int all = 0, before = 0;
         if (p.cache.rows > kKaThreads) {
-            all = ka_line<kKaThreads>(p, p.cache.rows, s_scan);  // already times streams
+            all = ka_line(p, s_scan);
             const int piece = ka_piece(all, p.ctas);
             if ((long long)blockIdx.x * piece >= all) return;
         }
