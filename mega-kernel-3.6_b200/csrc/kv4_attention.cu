@@ -130,10 +130,13 @@ template <>
 struct KaPair<__nv_bfloat16> {
     static constexpr unsigned kExponent = 0x7f80u, kTop = 255u;
     static constexpr int kShift = 7, kLeast = 23, kBias = 127;
-    // scales as f16, 2^(unit - bias) as 2^7: a shift of the exponents.  Scales 2^21 times smaller than that become 0.
+    // scales as f16, 2^(unit - bias) as 2: a shift of the exponents that makes 2^7 of it, then a product, which makes subnormals where they
+    // are due.  Scales 2^21 times smaller than that become 0.
     static __device__ __forceinline__ unsigned scales(unsigned w, int unit) {
         const unsigned c = (unsigned)(unit - 22) * 0x00800080u;
-        return __vmaxu2(w, c) * 8u - c * 8u;
+        const unsigned h = __vmaxu2(w, c) * 8u - c * 8u, f = 0x24002400u;  // 2^-6, twice
+        const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&f));
+        return *reinterpret_cast<const unsigned*>(&r);
     }
     static __device__ __forceinline__ unsigned pack(float x, float y) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
@@ -146,7 +149,7 @@ struct KaPair<__half> {
     static constexpr unsigned kExponent = 0x7c00u, kTop = 31u;
     static constexpr int kShift = 10, kLeast = 7, kBias = 15;
     static __device__ __forceinline__ unsigned scales(unsigned w, int unit) {
-        const unsigned f = (unsigned)(22 - unit + 15) * 0x04000400u;  // 2^(22 - unit), twice
+        const unsigned f = (unsigned)(16 - unit + 15) * 0x04000400u;  // 2^(16 - unit), twice
         const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&f));
         return *reinterpret_cast<const unsigned*>(&h);
     }
@@ -210,13 +213,13 @@ __device__ __forceinline__ unsigned ka_centred(unsigned code, int times) {
 // The least unit, and what a sum in units of it is multiplied by.
 template <typename T>
 __device__ __forceinline__ int ka_least_unit() {
-    if constexpr (sizeof(T) == 4) return 1;
+    if constexpr (sizeof(T) == 4) return 8;
     else return KaPair<T>::kLeast;
 }
 template <typename T>
 __device__ __forceinline__ float ka_unit_value(int unit) {
-    if constexpr (sizeof(T) == 4) return pow2(unit - 127);
-    else return pow2(unit - KaPair<T>::kBias - 7);
+    if constexpr (sizeof(T) == 4) return pow2(unit - 134);
+    else return pow2(unit - KaPair<T>::kBias - 1);
 }
 
 // Scales and zero points of a token's groups.
@@ -588,7 +591,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             transpose8(s[2], s[3]);
 
             // ---- scales of the values of the lane's four tokens.  The sums are kept in units of a scale's power of two, so that f16 holds
-            // weights times scales, and the unit is raised when a scale is 2^4 times larger (2^9 for fp32).  The exponents' bits or'ed
+            // weights times scales, and the unit is raised when a scale is 2^4 times larger.  The exponents' bits or'ed
             // together are no smaller than the largest; only where that says so, it is looked for.
             unsigned sw[2][G];  // two-byte types: pairs of tokens
             float vs[4][kWide ? G : 1], vz[4][kWide ? G : 1];
@@ -657,13 +660,13 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                         down = pow2(max(unit - largest, -126));
                         unit = largest;
                     }
-                    unit_limit = min(unit + (kWide ? 8 : 3), 254);  // the exponent of a NaN is always beyond it
+                    unit_limit = min(unit + 3, 254);  // the exponent of a NaN is always beyond it
                 }
                 const float m = fmaxf(top, most);
                 const float corr = m == -INFINITY ? 0.f : exp2f((top - m) * mult);  // nothing has been summed without a maximum
                 top = m;
                 limit_top = m == -INFINITY ? m : m + 4.f / mult;
-                shift = m == -INFINITY ? 0.f : -m * mult;
+                shift = m == -INFINITY ? 0.f : 6.f - m * mult;
                 weight_sum *= corr;
                 const float k0 = __shfl_sync(kFullMask, corr, 8 * j), k1 = __shfl_sync(kFullMask, corr, 8 * j + 4);
                 const float c0 = k0 * down, c1 = k1 * down;
@@ -682,7 +685,9 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                     }
             }
 
-            // fp32: the difference first, which is exact where it matters
+            // Weights, 2^6 times as large for the two-byte types (at most 2^10, and 2^5 for a scale, so that a product stays below 2^16): f16
+            // then holds those down to 2^-31 of the largest.  Many that small can be all there is, where the value of a key that draws
+            // nearly everything is 0.  fp32: the difference first, which is exact where it matters, and 2^7 goes into `shrink`.
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 s[i] = kWide ? exp2f((s[i] - (top == -INFINITY ? 0.f : top)) * mult) : exp2_approx(fmaf(s[i], mult, shift));
@@ -701,7 +706,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
 #pragma unroll
                         for (int gr = 0; gr < G; ++gr) {
                             const float2 f = KaPair<T>::unpack(sw[x][gr]);
-                            scale[x][gr] = pack_half(f.x * pow2(134 - unit), f.y * pow2(134 - unit));
+                            scale[x][gr] = pack_half(f.x * pow2(128 - unit), f.y * pow2(128 - unit));
                         }
                 }
                 unsigned z[4], za[2];
@@ -749,7 +754,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                         for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr], hi[gr][x], lo[gr][x]);
                 }
             } else {
-                const float shrink = pow2(127 - unit);
+                const float shrink = pow2(134 - unit);
                 weight_sum += (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {

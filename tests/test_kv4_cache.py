@@ -378,6 +378,36 @@ def test_attention_over_values_of_any_size(cuda_device, spread):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap", [12, 24, 26])
+def test_small_weights_count_where_the_largest_meets_zeros(cuda_device, dtype, gap):
+    """One key draws nearly everything and its value is 0, so that the output is made of weights near 2^-gap alone.  Weights, and weights
+    times scales, are held down to 2^-31 of the largest: a term is off by at most 2^-31 of its entry's size for either, and beyond that
+    as any term is."""
+    d, lengths = 64, [16, 200]
+    s = Server(cuda_device, dtype, d, 1, 32, lengths)
+    k, v = torch.randn(2, sum(lengths), 1, d, generator=torch.Generator().manual_seed(5)).mul(torch.tensor([0.01, 1.0]).view(2, 1, 1, 1)).to(dtype)
+    for sink in (3, 16 + 77):
+        k[sink], v[sink] = 1, 0
+    oracle.append(s.pool, s.table, s.lengths, k, v, s.lengths)
+    s.cache.pool.copy_(torch.from_numpy(s.pool))
+    q = torch.full((2, 8, d), gap * math.log(2) / math.sqrt(d)).to(dtype)
+    out = mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu).cpu().double()
+    for r, n in enumerate(lengths):
+        keys, values = (torch.as_tensor(x) for x in oracle.row_entries(s.pool, s.table[r], n, 0, d, dtype))
+        weight = torch.softmax(keys @ q[r].double().T / math.sqrt(d), 0)
+        size = values.abs().amax(1) * 3  # of an entry: |zero| + 15 scale, the least and the range of a group
+        want = weight.T @ values
+        score_size = (q[r].double().abs().sum(1) * keys.abs().max() / math.sqrt(d)) * 3
+        share = 2 * (score_size * 32 * 2.0**-22 + 2.0**-20)
+        limit = want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + ((weight.T @ size) * (share + (n / 16 + 8) * 2.0**-22) + n * 2.0**-30 * weight.amax(0) * size.max())[:, None]
+        if dtype is torch.float16:
+            limit = limit + 2.0**-25  # half a step of its subnormals
+        off = (out[r] - want).abs()
+        assert (off <= limit).all(), f"off by {(off / limit).max().item():.2f} of the limit"
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [1e-30, 1e-3, 12.0, 1e30])
 def test_attention_with_queries_of_any_size(cuda_device, size):
     s = Server(cuda_device, torch.bfloat16, 64, 2, 16, [77])
