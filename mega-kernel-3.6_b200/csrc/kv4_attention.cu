@@ -24,7 +24,7 @@
 // What bounds it.  Short rows: latency, 9.6 us for one row of 700 tokens.  Many long rows: not memory (tiles that all lie in L2 take 97 % of
 // the time) but the SMs: 626 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
 // of 8 cycles; issue slots, that pipe, the tensor cores and shared memory are each 40 to 60 % busy, with three warps a scheduler.  48 rows
-// of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78 us, 3.5 TB/s; 24 / 4 heads, three tokens, 12 rows: 42.8 us.
+// of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78 us, 3.5 TB/s; 24 / 4 heads, three tokens, 12 rows: 43.1 us.
 #include <math.h>
 
 #include <type_traits>
@@ -48,7 +48,7 @@ struct Kv4AttnParams {
     int query_heads, tokens, group, columns;  // group: query heads of a KV head; columns: group * tokens
     int blocks;                               // of eight columns
     int streams;                              // kv_heads * blocks: passes over a row
-    int ctas, wide_q, join_parts, join_threads;
+    int ctas, wide_q, join_wide;
     float scale;
     FastDiv fd_blocks, fd_group, fd_streams;
 };
@@ -259,23 +259,74 @@ __device__ __forceinline__ void ka_advance(const Kv4AttnParams& p, KaCursor& c, 
     }
 }
 
-// Tiles of the whole line, below 2^31 as the host sees to.  Every thread of the attention kernel calls it; s: a word for each warp.
+// All CTAs, and the join, cut the line alike.
+__device__ __forceinline__ int ka_piece(int total, int ctas) {
+    return max(kKaMinTiles, (int)(((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas));
+}
+
+// Tiles of the whole line, below 2^31 as the host sees to.  Every thread of a CTA calls it; s: a word for each warp.
+template <int kWarps>
 __device__ __forceinline__ int ka_line(const Kv4AttnParams& p, int* s) {
     int mine = 0;
-    for (int r = threadIdx.x; r < p.cache.rows; r += kKaThreads) mine += ka_tiles(p.cache, r);
+    for (int r = threadIdx.x; r < p.cache.rows; r += kWarps * 32) mine += ka_tiles(p.cache, r);
     mine = __reduce_add_sync(kFullMask, mine);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = mine;
     __syncthreads();
     int sum = 0;
 #pragma unroll
-    for (int w = 0; w < kKaWarps; ++w) sum += s[w];
+    for (int w = 0; w < kWarps; ++w) sum += s[w];
     return sum * p.streams;
 }
 
-// All CTAs, and the join, cut the line alike.
-__device__ __forceinline__ int ka_piece(int total, int ctas) {
-    return max(kKaMinTiles, (int)(((unsigned)total + (unsigned)ctas - 1u) / (unsigned)ctas));
+// The piece [begin, end) of the line that belongs to CTA `cta`, and the tile it begins at; false where nothing is left for that CTA.  Every
+// thread of a CTA calls it; s: a word for each warp, and three.
+template <int kWarps>
+__device__ __forceinline__ bool ka_begin(const Kv4AttnParams& p, int cta, int* s, int& piece, int& begin, int& end, KaCursor& start) {
+    constexpr int kThreads = kWarps * 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *s_scan = s, *s_start = s + kWarps;
+    int all = 0, before = 0;
+    if (p.cache.rows > kThreads) {
+        all = ka_line<kWarps>(p, s_scan);
+        piece = ka_piece(all, p.ctas);
+        if ((long long)cta * piece >= all) return false;
+    }
+    for (int base = 0;; base += kThreads) {  // rows in batches of a thread each
+        const int r = base + threadIdx.x;
+        const int n = r < p.cache.rows ? ka_tiles(p.cache, r) : 0;
+        int inc = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int x = __shfl_up_sync(kFullMask, inc, off);
+            if (lane >= off) inc += x;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp] = inc;
+        __syncthreads();
+        int batch = 0, lower = before;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) lower += s_scan[w];
+            batch += s_scan[w];
+        }
+        if (p.cache.rows <= kThreads) all = batch * p.streams;
+        piece = ka_piece(all, p.ctas);
+        if ((long long)cta * piece >= all) return false;  // the whole CTA, in its first batch
+        begin = cta * piece, end = all - begin < piece ? all : begin + piece;
+        // begin's row has first * streams <= begin < (first + n) * streams
+        const int target = fdiv(begin, p.fd_streams), first = lower + inc - n;
+        if (first <= target && target < first + n) s_start[0] = r, s_start[1] = first, s_start[2] = n;
+        before += batch;
+        if (before > target || base + kThreads >= p.cache.rows) break;
+    }
+    __syncthreads();
+    start.row = s_start[0];
+    start.tiles = s_start[2];
+    const int off = begin - s_start[1] * p.streams;
+    start.stream = (unsigned)off / (unsigned)start.tiles;
+    start.tile = off - start.stream * start.tiles;
+    return true;
 }
 
 template <typename T, int D>
@@ -284,7 +335,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
     constexpr int G = C::kGroups, QP = C::kQParts;
     constexpr bool kWide = sizeof(T) == 4;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int s_scan[kKaWarps], s_start[3], s_abort;
+    __shared__ int s_scan[kKaWarps + 3], s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
     unsigned char* ring = smem + warp * C::kStages * C::kTile;
     float* s_fold = reinterpret_cast<float*>(smem + kKaWarps * C::kStages * C::kTile);
@@ -301,49 +352,11 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
     if (threadIdx.x == 0) s_abort = 0;
     asm volatile("griddepcontrol.launch_dependents;");  // the join may be set up while this runs; it waits for the end of the grid
 
-    // ---- this CTA's piece of the line, and the row it begins in: begin's row has before * streams <= begin < (before + tiles) * streams
     int begin, end;
     KaCursor start;
     {
-        int all = 0, before = 0;
-        if (p.cache.rows > kKaThreads) {
-            all = ka_line(p, s_scan);
-            const int piece = ka_piece(all, p.ctas);
-            if ((long long)blockIdx.x * piece >= all) return;
-        }
-        for (int base = 0;; base += kKaThreads) {  // rows in batches of a thread each
-            const int r = base + threadIdx.x;
-            const int n = r < p.cache.rows ? ka_tiles(p.cache, r) : 0;
-            int inc = n;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int x = __shfl_up_sync(kFullMask, inc, off);
-                if (lane >= off) inc += x;
-            }
-            __syncthreads();
-            if (lane == 31) s_scan[warp] = inc;
-            __syncthreads();
-            int batch = 0, lower = before;
-#pragma unroll
-            for (int w = 0; w < kKaWarps; ++w) {
-                if (w < warp) lower += s_scan[w];
-                batch += s_scan[w];
-            }
-            if (p.cache.rows <= kKaThreads) all = batch * p.streams;
-            const int piece = ka_piece(all, p.ctas);
-            if ((long long)blockIdx.x * piece >= all) return;  // the whole CTA, in its first batch
-            begin = blockIdx.x * piece, end = all - begin < piece ? all : begin + piece;
-            const int target = fdiv(begin, p.fd_streams), first = lower + inc - n;
-            if (first <= target && target < first + n) s_start[0] = r, s_start[1] = first, s_start[2] = n;
-            before += batch;
-            if (before > target || base + kKaThreads >= p.cache.rows) break;
-        }
-        __syncthreads();
-        start.row = s_start[0];
-        start.tiles = s_start[2];
-        const int off = begin - s_start[1] * p.streams;
-        start.stream = (unsigned)off / (unsigned)start.tiles;
-        start.tile = off - start.stream * start.tiles;
+        int piece;
+        if (!ka_begin<kKaWarps>(p, blockIdx.x, s_scan, piece, begin, end, start)) return;
     }
 
     // A warp prepares one group of 64 channels of every column's query (lane: column g, channels 16 j .. + 15).  They are requested a
@@ -899,39 +912,67 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
     }
 }
 
-// Joins the partial results of rows that several CTAs worked on; rows without a token get zeros.  A CTA takes a query head and token, or 64
-// channels of it (p.join_parts CTAs for an output).  A warp takes 64 channels of every few partial results, kBatch of them in flight
-// together, with a running maximum of its own.  A round trip for a batch is 2 to 3 us, so few outputs get more warps: one row of
-// 32768 tokens, 74 partial results for each head, 17.7 us for the call with one batch of 32 warps, 23.9 with two of eight.
+// Adds partial results (maximum and sum of weights; sums of two channels) to what a warp has so far.
+template <int N>
+__device__ __forceinline__ void ka_join(const float2 (&stats)[N], const float2 (&value)[N], float& top, float& sum, float2& acc) {
+    float now = top;
+#pragma unroll
+    for (int i = 0; i < N; ++i) now = fmaxf(now, stats[i].x);
+    const float base = now == -INFINITY ? 0.f : now, corr = exp2f(top - base);
+    sum *= corr, acc.x *= corr, acc.y *= corr;
+    top = now;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float own = exp2f(stats[i].x - base);
+        sum += stats[i].x == -INFINITY ? stats[i].y : own * stats[i].y;  // without a maximum the sum is 0 or NaN
+        acc.x = fmaf(own, value[i].x, acc.x), acc.y = fmaf(own, value[i].y, acc.y);
+    }
+}
+
+// The same for the partial results of the CTAs c0, c0 + step, ... up to cta1: kBatch of them, all requested at once.
+template <int kBatch, int D>
+__device__ __forceinline__ void ka_join_batch(const float* values, const float* both, int first, int piece, int c0, int step, int cta1, int lane,
+                                              float& top, float& sum, float2& acc) {
+    float2 stats[kBatch], value[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const int c = min(c0 + i * step, cta1);  // loads without a branch; one too many counts for nothing
+        const long long slot = (2ll * c + (first > c * piece ? 1 : 0)) * ka_slot_floats(D);
+        stats[i] = __ldcg(reinterpret_cast<const float2*>(both + slot));
+        value[i] = __ldcg(reinterpret_cast<const float2*>(values + slot) + lane);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+        if (c0 + i * step > cta1) stats[i] = make_float2(-INFINITY, 0.f), value[i] = make_float2(0.f, 0.f);
+    ka_join<kBatch>(stats, value, top, sum, acc);
+}
+
+// Joins the partial results of passes that several CTAs worked on; rows without a token get zeros.  Two forms, as ka_grid chooses: few
+// passes, cut into very many pieces, or any others.
+//
+// Few passes: a CTA of 32 warps takes 64 channels of one query head and token.  A warp takes every 32nd partial result, kBatch of them in
+// flight together, with a running maximum of its own: a round trip for a batch is 2 to 3 us (one row of 32768 tokens, 16 / 2 heads of 256,
+// 205 partial results for each: 16.7 us for the call, 19.1 with the other form; one of 700 tokens 8.8 and 9.0).
+constexpr int kKaWideWarps = 32;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(1024) kv4_attention_join_kernel(const __grid_constant__ Kv4AttnParams p) {
-    constexpr int kBatch = 3, kParts = D / 64;
-    __shared__ float2 s_out[32][32];
-    __shared__ float s_max[32], s_sum[32];
-    __shared__ int s_scan[32], s_before[32];
-    const int warps = blockDim.x / 32;
+__global__ void __launch_bounds__(kKaWideWarps * 32) kv4_attention_join_wide_kernel(const __grid_constant__ Kv4AttnParams p) {
+    constexpr int kBatch = 4, kParts = D / 64;  // 4: with 3, 32 registers, two CTAs crowd on an SM (18.8 us instead of 16.7)
+    __shared__ float2 s_out[kKaWideWarps][32];
+    __shared__ float s_max[kKaWideWarps], s_sum[kKaWideWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool split = p.join_parts > 1;
-    const int output = split ? blockIdx.x / kParts : blockIdx.x;
-    const int part = split ? blockIdx.x % kParts : warp % kParts;
-    const int turn = split ? warp : warp / kParts, turns = split ? warps : warps / kParts;
+    const int output = blockIdx.x / kParts, part = blockIdx.x % kParts;
     const int head = output % p.query_heads, rest = output / p.query_heads;
     const int token = rest % p.tokens, row = rest / p.tokens;
     T* out = static_cast<T*>(p.out) + (long long)output * D + part * 64;
-    // tiles of the rows before this one, and of all rows
-    int mine = 0, mine_before = 0;
-    for (int r = threadIdx.x; r < p.cache.rows; r += blockDim.x) {
+    int mine = 0, mine_before = 0;  // tiles of all rows, and of those before this one; every warp sums them up
+    for (int r = lane; r < p.cache.rows; r += 32) {
         const int n = ka_tiles(p.cache, r);
         mine += n;
         mine_before += r < row ? n : 0;
     }
     const int tiles = ka_tiles(p.cache, row);
-    mine = __reduce_add_sync(kFullMask, mine);
-    mine_before = __reduce_add_sync(kFullMask, mine_before);
-    if (lane == 0) s_scan[warp] = mine, s_before[warp] = mine_before;
-    __syncthreads();
-    const int total = __reduce_add_sync(kFullMask, lane < warps ? s_scan[lane] : 0) * p.streams;
-    const int before = __reduce_add_sync(kFullMask, lane < warps ? s_before[lane] : 0) * p.streams;
+    const int total = __reduce_add_sync(kFullMask, mine) * p.streams, before = __reduce_add_sync(kFullMask, mine_before) * p.streams;
     const int kv_head = fdiv(head, p.fd_group), column = token * p.group + head - kv_head * p.group;
     const int block = column / 8;
     const int piece = ka_piece(total, p.ctas);
@@ -939,58 +980,91 @@ __global__ void __launch_bounds__(1024) kv4_attention_join_kernel(const __grid_c
     const int cta0 = (unsigned)first / (unsigned)piece, cta1 = (unsigned)(first + max(tiles, 1) - 1) / (unsigned)piece;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // no CTA of this grid ends before the grid ahead of it
     if (tiles == 0) {
-        if (turn == 0) out[2 * lane] = out[2 * lane + 1] = from_float<T>(0.f);
+        if (warp == 0) out[2 * lane] = out[2 * lane + 1] = from_float<T>(0.f);
         return;
     }
     if (cta0 == cta1) return;  // that CTA has written the output
     const float* base = p.partial + (column - block * 8) * (D + 4);
     float top = -INFINITY, sum = 0.f;
     float2 acc = make_float2(0.f, 0.f);
-    for (int c0 = cta0 + turn; c0 <= cta1; c0 += turns * kBatch) {
-        float2 stats[kBatch], value[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int c = min(c0 + i * turns, cta1);  // loads without a branch are all on their way at once; one too many counts for nothing
-            const float* x = base + (2ll * c + (first > c * piece ? 1 : 0)) * ka_slot_floats(D);
-            stats[i] = __ldcg(reinterpret_cast<const float2*>(x + D));
-            value[i] = __ldcg(reinterpret_cast<const float2*>(x + part * 64) + lane);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (c0 + i * turns > cta1) stats[i] = make_float2(-INFINITY, 0.f), value[i] = make_float2(0.f, 0.f);
-        float now = top;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) now = fmaxf(now, stats[i].x);
-        const float base_now = now == -INFINITY ? 0.f : now, corr = exp2f(top - base_now);
-        sum *= corr, acc.x *= corr, acc.y *= corr;
-        top = now;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const float own = exp2f(stats[i].x - base_now);
-            sum += stats[i].x == -INFINITY ? stats[i].y : own * stats[i].y;  // without a maximum the sum is 0 or NaN
-            acc.x = fmaf(own, value[i].x, acc.x), acc.y = fmaf(own, value[i].y, acc.y);
-        }
-    }
+    for (int c0 = cta0 + warp; c0 <= cta1; c0 += kKaWideWarps * kBatch)
+        ka_join_batch<kBatch, D>(base + part * 64, base + D, first, piece, c0, kKaWideWarps, cta1, lane, top, sum, acc);
     s_out[warp][lane] = acc;
     if (lane == 0) s_max[warp] = top, s_sum[warp] = sum;
     __syncthreads();
-    if (turn != 0) return;
-    // the warps of this part: warp, warp + step, ...; each lane looks at one of them
-    const int step = split ? 1 : kParts, peer = warp + lane * step;
-    const float peer_max = peer < warps ? s_max[peer] : -INFINITY, peer_sum = peer < warps ? s_sum[peer] : 0.f;
+    if (warp != 0) return;
+    const float peer_max = s_max[lane], peer_sum = s_sum[lane];  // each lane looks at one of the warps
     const float all_top = warp_max(peer_max);
     const float peer_own = peer_max == -INFINITY ? 0.f : exp2f(peer_max - all_top);
     const float all = warp_sum(peer_max == -INFINITY ? peer_sum : peer_own * peer_sum);
     float2 value = make_float2(0.f, 0.f);
 #pragma unroll 8
-    for (int i = 0; i < turns; ++i) {
+    for (int i = 0; i < kKaWideWarps; ++i) {
         const float own = __shfl_sync(kFullMask, peer_own, i);
-        const float2 x = s_out[warp + i * step][lane];
+        const float2 x = s_out[i][lane];
         value.x = fmaf(own, x.x, value.x), value.y = fmaf(own, x.y, value.y);
     }
     const float inv = all == 0.f ? 0.f : 1.f / all;
     out[2 * lane] = from_float<T>(all == 0.f ? 0.f : value.x * inv);
     out[2 * lane + 1] = from_float<T>(all == 0.f ? 0.f : value.y * inv);
+}
+
+// Any others: a CTA for each cut of the line, and those of one pass share its eight columns and their groups of 64 channels.  Passes that
+// are whole cost nothing (a CTA for each query head took 35 us where this takes 26: 256 rows of 500 tokens, 16 / 2 heads of 128; 57 and 24
+// for 1024 rows of 7).  With eight partial results in flight for a warp, not three, 74 registers leave room for three CTAs an SM: 30 us.
+constexpr int kKaJoinWarps = 8;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kKaJoinWarps * 32) kv4_attention_join_cuts_kernel(const __grid_constant__ Kv4AttnParams p) {
+    constexpr int kBatch = 3, kParts = D / 64, kItems = 8 * kParts;
+    __shared__ float2 s_out[kKaJoinWarps][32];
+    __shared__ float s_max[kKaJoinWarps], s_sum[kKaJoinWarps];
+    __shared__ int s_scan[kKaJoinWarps + 3];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int piece, begin, end;
+    KaCursor start;
+    const bool cut = ka_begin<kKaJoinWarps>(p, blockIdx.x, s_scan, piece, begin, end, start) && start.tile > 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // no CTA of this grid ends before the grid ahead of it
+    for (int row = blockIdx.x; row < p.cache.rows; row += gridDim.x) {
+        if (ka_tiles(p.cache, row) != 0) continue;
+        const long long n = (long long)p.tokens * p.query_heads * D;
+        T* out = static_cast<T*>(p.out) + row * n;
+        for (long long i = threadIdx.x; i < n; i += kKaJoinWarps * 32) out[i] = from_float<T>(0.f);
+    }
+    if (!cut) return;
+    const int first = begin - start.tile, cta0 = (unsigned)first / (unsigned)piece, cta1 = (unsigned)(first + start.tiles - 1) / (unsigned)piece;
+    const int share = min(1 << (31 - __clz(cta1 - cta0)), kItems);  // CTAs that work on the segment
+    const int index = blockIdx.x - cta0 - 1;
+    if (index >= share) return;
+    const int items = kItems / share, turns = max(kKaJoinWarps / items, 1), turn = warp % turns;
+    const int kv_head = fdiv(start.stream, p.fd_blocks), block = start.stream - kv_head * p.blocks;
+    for (int i = warp / turns; i < items; i += kKaJoinWarps / turns) {  // more than once only where turns is 1
+        const int item = index * items + i, mine = item / kParts, part = item % kParts, column = block * 8 + mine;
+        const float* base = p.partial + mine * (D + 4);
+        float top = -INFINITY, sum = 0.f;
+        float2 acc = make_float2(0.f, 0.f);
+        for (int c0 = cta0 + turn; c0 <= cta1 && column < p.columns; c0 += turns * kBatch)
+            ka_join_batch<kBatch, D>(base + part * 64, base + D, first, piece, c0, turns, cta1, lane, top, sum, acc);
+        if (turns > 1) {
+            s_out[warp][lane] = acc;
+            if (lane == 0) s_max[warp] = top, s_sum[warp] = sum;
+            __syncthreads();
+            if (turn == 0) {
+                float2 stats[1], value[1];
+                for (int w = warp + 1; w < warp + turns; ++w) {
+                    stats[0] = make_float2(s_max[w], s_sum[w]), value[0] = s_out[w][lane];
+                    ka_join<1>(stats, value, top, sum, acc);
+                }
+            }
+        }
+        if (turn == 0 && column < p.columns) {
+            const int token = fdiv(column, p.fd_group), head = kv_head * p.group + column - token * p.group;
+            T* out = static_cast<T*>(p.out) + (((long long)start.row * p.tokens + token) * p.query_heads + head) * D + part * 64;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            out[2 * lane] = from_float<T>(sum == 0.f ? 0.f : acc.x * inv);
+            out[2 * lane + 1] = from_float<T>(sum == 0.f ? 0.f : acc.y * inv);
+        }
+    }
 }
 
 static int kv4_attention_params(const mk36_kv4_cache* c, const mk36_kv4_attention_args* a, Kv4AttnParams* p) {
@@ -1028,15 +1102,16 @@ static int ka_grid(Kv4AttnParams* p, const mk36_kv4_cache* c) {
     p->blocks = (p->columns + 7) / 8;
     p->streams = p->cache.kv_heads * p->blocks;
     p->fd_blocks = make_fastdiv((unsigned)p->blocks), p->fd_group = make_fastdiv((unsigned)p->group), p->fd_streams = make_fastdiv((unsigned)p->streams);
-    // 1024 threads for an output, and a CTA for 64 of its channels, as long as that is no more than two such CTAs for each SM
-    const long long outputs = (long long)p->cache.rows * p->tokens * p->query_heads;
-    p->join_threads = outputs <= 2 * info->sm_count ? 1024 : 256;
-    p->join_parts = outputs * (c->head_dim / 64) <= 2 * info->sm_count ? c->head_dim / 64 : 1;
     const double line = (double)p->cache.rows * p->cache.row_pages * (c->page_size / kKv4Tile) * p->streams;
     if (line > 2e9) MK36_FAIL(MK36_ERR_UNSUPPORTED, "kv4_attention_decode: the table holds more than 2e9 tiles of 16 tokens, heads and query blocks");
     const long long most = (long long)line;
     const long long ctas = (most + kKaMinTiles - 1) / kKaMinTiles, resident = (long long)info->sm_count * ka_ctas_per_sm(c->dtype == MK36_F32, c->head_dim);
     p->ctas = (int)(ctas < resident ? ctas : resident);
+    // The wide form of the join: more than 64 pieces a pass when the table is full (4 rows, 16 / 2 heads of 128, 74 pieces: 15.0 us, 17.0 with
+    // the other; 2 rows, 24 / 4 heads of 256, 55 pieces: 30.4 and 30.2), or an SM for each CTA of both launches.  Either way there
+    // are at most two such CTAs for each SM.
+    const long long outputs = (long long)p->cache.rows * p->tokens * p->query_heads;
+    p->join_wide = p->ctas > 64ll * p->cache.rows * p->streams || p->ctas + outputs * (c->head_dim / 64) <= info->sm_count;
     return MK36_OK;
 }
 
@@ -1048,15 +1123,15 @@ static int kv4_attention_launch(const Kv4AttnParams& p, cudaStream_t s) {
     kv4_attention_kernel<T, D><<<p.ctas, kKaThreads, C::kSmem, s>>>(p);
     MK36_CUDA_OK(cudaGetLastError());
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)((long long)p.cache.rows * p.tokens * p.query_heads * p.join_parts));
-    config.blockDim = dim3(p.join_threads);
+    config.gridDim = dim3(p.join_wide ? (unsigned)(p.cache.rows * p.tokens * p.query_heads * (D / 64)) : (unsigned)p.ctas);
+    config.blockDim = dim3(p.join_wide ? kKaWideWarps * 32 : kKaJoinWarps * 32);
     config.stream = s;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
-    MK36_CUDA_OK(cudaLaunchKernelEx(&config, kv4_attention_join_kernel<T, D>, p));
+    MK36_CUDA_OK(cudaLaunchKernelEx(&config, p.join_wide ? kv4_attention_join_wide_kernel<T, D> : kv4_attention_join_cuts_kernel<T, D>, p));
     return MK36_OK;
 }
 

@@ -487,6 +487,21 @@ def test_long_ragged_batch_and_lengths_out_of_range(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,hq,hkv,tokens", [(64, 8, 1, 1), (64, 3, 3, 2), (128, 12, 2, 1), (256, 16, 2, 1), (256, 5, 1, 3)])
+def test_passes_cut_into_any_number_of_pieces(cuda_device, dtype, d, hq, hkv, tokens):
+    for lengths in ([2500, 0, 100, 200, 5, 400, 0, 64, 65, 900, 130, 17, 0], [1700], [300, 260]):
+        s = Server(cuda_device, dtype, d, hkv, 64, lengths, seed=len(lengths))
+        s.fill(seed=d)
+        q = torch.randn(len(lengths), tokens, hq, d, generator=torch.Generator().manual_seed(11)).to(dtype)
+        for width in (s.gpu.pages.shape[1], 2000):  # the same rows in a table with room for far more
+            pages = torch.full((len(lengths), width), -1, dtype=torch.int32, device=cuda_device)
+            pages[:, : s.gpu.pages.shape[1]] = s.gpu.pages
+            del [torch.full((1 << k,), float("nan"), device=cuda_device) for k in range(6, 22)][:]  # what an output not written may hold
+            check_attention(s, q, mk.kv4_attention_decode(q.to(cuda_device), s.cache, mk.PageTable(pages, s.gpu.lengths, s.gpu.refcounts)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [129, 300])
 def test_more_rows_than_threads(cuda_device, rows):
     lengths = [(r * 7) % 40 for r in range(rows)]
