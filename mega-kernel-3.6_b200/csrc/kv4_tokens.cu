@@ -8,7 +8,7 @@
 // Codes and scales follow from exact arithmetic, whatever the order of operations in fp32 would give: see codes_of and scale_of.
 //
 // What bounds them: reading back, memory and instructions alike (32768 tokens of 2 heads of 256 in bf16: 83 MB in 16.3 us, 5.1 TB/s);
-// appending, instructions, about 150 for 16 values (31.5 us, 2.7 TB/s; 27.8 us in f16, where fewer values lie half way between codes).
+// appending, instructions (28.7 us, 2.9 TB/s; 26.2 us in f16, where fewer values lie half way between codes).
 #include <type_traits>
 
 #include "mk36_kv4.cuh"
@@ -139,6 +139,26 @@ __device__ __forceinline__ unsigned codes_exact(const float (&x)[8], float zero,
     return four_exact(make_float4(x[0], x[1], x[2], x[3]), zero, scale) | four_exact(make_float4(x[4], x[5], x[6], x[7]), zero, scale) << 16;
 }
 
+// Two fp32 operations an instruction, each rounded as one alone would be.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float x, float y) {
+    f32x2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ float first_of(f32x2 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float second_of(f32x2 v) { return __uint_as_float((unsigned)(v >> 32)); }
+__device__ __forceinline__ f32x2 add_pair(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 fma_pair(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 constexpr float kRoundUp = 12582912.0f;  // 1.5 * 2^23: added, it rounds to a whole number, halves to even, and leaves that in the low bits
 
 // Whole numbers below 16, as floats, to a word of eight half bytes: sums of four are exact.
@@ -154,16 +174,23 @@ __device__ __forceinline__ unsigned pack_codes(const float (&n)[8]) {
 template <typename T>
 __device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, float scale, float inv, const T*) {
     const float half = 0.5f * scale;
+    const f32x2 zeros = pair_of(-zero, -zero), scales = pair_of(-scale, -scale), invs = pair_of(inv, inv), up = pair_of(kRoundUp, kRoundUp),
+                down = pair_of(-kRoundUp, -kRoundUp);
     float n[8], r[8];
+    f32x2 m[4];  // n of i and i + 4
     bool border = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float d = x[i] - zero;
-        n[i] = fmaf(d, inv, kRoundUp) - kRoundUp;
-        r[i] = fmaf(-n[i], scale, d);
+    for (int i = 0; i < 4; ++i) {
+        const f32x2 d = add_pair(pair_of(x[i], x[i + 4]), zeros);
+        m[i] = add_pair(fma_pair(d, invs, up), down);
+        const f32x2 rest = fma_pair(m[i], scales, d);
+        r[i] = first_of(rest), r[i + 4] = second_of(rest);
         border |= fabsf(r[i]) >= half;
+        border |= fabsf(r[i + 4]) >= half;
     }
     if (border) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n[i] = first_of(m[i]), n[i + 4] = second_of(m[i]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (fabsf(r[i]) >= half) {
@@ -173,8 +200,12 @@ __device__ __forceinline__ unsigned codes_of(const float (&x)[8], float zero, fl
                 if (over > 0.0f || (over == 0.0f && odd)) n[i] += way;
             }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[i] = pair_of(n[i], n[i + 4]);
     }
-    return pack_codes(n);
+    // the word's two halves at once: sums of four whole numbers below 16 are exact
+    const f32x2 word = add_pair(fma_pair(m[3], pair_of(4096.0f, 4096.0f), fma_pair(m[2], pair_of(256.0f, 256.0f), fma_pair(m[1], pair_of(16.0f, 16.0f), m[0]))), up);
+    return __byte_perm(__float_as_uint(first_of(word)), __float_as_uint(second_of(word)), 0x5410);
 }
 
 // Codes of fp32 values: neither the difference nor the product is exact, so near a border fp64 decides.  The quotient is off by less than
@@ -258,7 +289,7 @@ __device__ __forceinline__ void write_param(unsigned char* p, float scale, float
 // A token has pieces of 8 channels (read) or 16 (append): keys of all heads, then values.  A CTA takes p.cta_tokens consecutive tokens
 // and 32 of the pieces: a lane keeps its piece, a warp takes every fourth token.  Where a token's codes go is looked up once, by one
 // thread.
-constexpr int kTokThreads = 128, kTokWarps = kTokThreads / 32, kMaxCtaTokens = 32, kBatch = 2;  // kBatch: loads of a lane that are on their way together
+constexpr int kTokThreads = 128, kTokWarps = kTokThreads / 32, kMaxCtaTokens = 32, kBatch = 2;  // kBatch: loads of a lane of the read that are on their way together
 
 struct Kv4Where {
     long long dense[2];      // elements from the start of k and of v
@@ -318,48 +349,47 @@ struct Kv4Piece {
     __device__ __forceinline__ unsigned char* param_at(int token) const { return where[token].param + param; }
 };
 
+// A warp requests its next token before it works on this one; 64 registers (two-byte types), eight CTAs an SM (32768 tokens: 28.7 us; two tokens requested and
+// then worked on, 29.6, and 31.4 with one fp32 operation an instruction).
 template <typename T, int D>
-__global__ void __launch_bounds__(kTokThreads) kv4_append_kernel(const __grid_constant__ Kv4TokenParams p) {
+__global__ void __launch_bounds__(kTokThreads, sizeof(T) == 4 ? 6 : 8) kv4_append_kernel(const __grid_constant__ Kv4TokenParams p) {
     __shared__ Kv4Where s_where[kMaxCtaTokens];
     if ((int)threadIdx.x < p.cta_tokens) kv4_find<T, D>(p, (long long)blockIdx.x * p.cta_tokens + threadIdx.x, s_where[threadIdx.x]);
     const Kv4Piece<T, D, 16> piece(p, s_where);  // four lanes have a group
     __syncthreads();
+    Chunk8<T> next[2];
+    auto request = [&](int token) {
+        zero_chunk8<T>(next[0]);
+        zero_chunk8<T>(next[1]);
+        if (token < p.cta_tokens && piece.there && s_where[token].param) {
+            const T* src = piece.dense_at(token);
+            next[0] = load8<T>(src, p.wide != 0);
+            next[1] = load8<T>(src + 8, p.wide != 0);
+        }
+    };
+    request(threadIdx.x >> 5);
 #pragma unroll 1
-    for (int first = threadIdx.x >> 5; first < p.cta_tokens; first += kTokWarps * kBatch) {
-        Chunk8<T> chunk[kBatch][2];
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const int token = first + b * kTokWarps;
-            zero_chunk8<T>(chunk[b][0]);
-            zero_chunk8<T>(chunk[b][1]);
-            if (token < p.cta_tokens && piece.there && s_where[token].param) {
-                const T* src = piece.dense_at(token);
-                chunk[b][0] = load8<T>(src, p.wide != 0);
-                chunk[b][1] = load8<T>(src + 8, p.wide != 0);
-            }
+    for (int token = threadIdx.x >> 5; token < p.cta_tokens; token += kTokWarps) {
+        const Chunk8<T> chunk[2] = {next[0], next[1]};
+        request(token + kTokWarps);  // on its way while this one is worked on
+        if (!s_where[token].param) continue;  // all of the warp
+        float f[16], low, high;
+        unpack8(chunk[0], *reinterpret_cast<float(*)[8]>(&f[0]));
+        unpack8(chunk[1], *reinterpret_cast<float(*)[8]>(&f[8]));
+        least_greatest(f, chunk, low, high);
+        const bool fine = fabsf(low) < INFINITY && fabsf(high) < INFINITY;
+        const float zero = low + 0.0f;  // -0 becomes 0
+        const float scale = fine ? scale_of(low, high, static_cast<const T*>(nullptr)) : 0.0f;
+        const uint2 words = two_words<T>(f, zero, high, scale);
+        __syncwarp();
+        if (!piece.there) continue;
+        if (piece.of == 0) {
+            *reinterpret_cast<uint2*>(piece.word_at(token)) = words;
+        } else {
+            piece.word_at(token)[0] = words.x;
+            piece.word_at(token)[D / 16] = words.y;  // four units on: the next eight channels' lane
         }
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const int token = first + b * kTokWarps;
-            if (token >= p.cta_tokens || !s_where[token].param) continue;  // all of the warp
-            float f[16], low, high;
-            unpack8(chunk[b][0], *reinterpret_cast<float(*)[8]>(&f[0]));
-            unpack8(chunk[b][1], *reinterpret_cast<float(*)[8]>(&f[8]));
-            least_greatest(f, chunk[b], low, high);
-            const bool fine = fabsf(low) < INFINITY && fabsf(high) < INFINITY;
-            const float zero = low + 0.0f;  // -0 becomes 0
-            const float scale = fine ? scale_of(low, high, static_cast<const T*>(nullptr)) : 0.0f;
-            const uint2 words = two_words<T>(f, zero, high, scale);
-            __syncwarp();
-            if (!piece.there) continue;
-            if (piece.of == 0) {
-                *reinterpret_cast<uint2*>(piece.word_at(token)) = words;
-            } else {
-                piece.word_at(token)[0] = words.x;
-                piece.word_at(token)[D / 16] = words.y;  // four units on: the next eight channels' lane
-            }
-            if (threadIdx.x % 4 == 0) write_param<T>(piece.param_at(token), scale, zero, fine);
-        }
+        if (threadIdx.x % 4 == 0) write_param<T>(piece.param_at(token), scale, zero, fine);
     }
 }
 
