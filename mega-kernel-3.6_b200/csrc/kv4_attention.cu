@@ -22,7 +22,7 @@
 // leaves a partial result, and a second launch, set up while the first still runs, joins those.
 //
 // What bounds it.  Short rows: latency, 9.6 us for one row of 700 tokens.  Many long rows: not memory (tiles that all lie in L2 take 97 % of
-// the time) but the SMs: 626 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
+// the time) but the SMs: 632 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
 // of 8 cycles; issue slots, that pipe, the tensor cores and shared memory are each 40 to 60 % busy, with three warps a scheduler.  48 rows
 // of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78 us, 3.5 TB/s; 24 / 4 heads, three tokens, 12 rows: 43.1 us.
 #include <math.h>
