@@ -772,6 +772,32 @@ def test_calls_on_two_streams_and_two_captured_graphs_do_not_meet(cuda_device):
 
 
 @pytest.mark.gpu
+def test_calls_without_tokens_and_in_inference_mode(cuda_device):
+    s = Server(cuda_device, torch.bfloat16, 64, 2, 16, [20, 0])
+    s.fill()
+    none = torch.empty(2, 0, 2, 64, dtype=torch.bfloat16, device=cuda_device)
+    mk.kv4_append(s.cache, s.gpu, none, none)
+    mk.kv4_append(s.cache, s.gpu, none[0], none[0], cu_tokens=_cu([0, 0], cuda_device))
+    s.same_pool()
+    for k, v in (mk.kv4_read(s.cache, s.gpu, 0), mk.kv4_read(s.cache, s.gpu, 0, cu_tokens=_cu([0, 0], cuda_device))):
+        assert k.numel() == v.numel() == 0 and k.shape == v.shape
+    nobody = torch.empty(0, dtype=torch.int32, device=cuda_device)
+    same, status = mk.kv_pages_fork(s.gpu, nobody, nobody)
+    assert status.item() == 0 and _lists(same) == _lists(s.gpu)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(2)).bfloat16().to(cuda_device)
+    with torch.inference_mode():
+        longer, status = mk.kv_pages_resize(s.cache, s.gpu, s.gpu.lengths + 1)
+        k = torch.ones(2, 1, 2, 64, dtype=torch.bfloat16, device=cuda_device)
+        mk.kv4_append(s.cache, longer, k, k)
+        assert status.item() == 0
+        out = mk.kv4_attention_decode(q, s.cache, longer)
+        assert torch.equal(mk.kv4_read(s.cache, longer, 1)[1], k)
+        mk.kv_pages_compact(s.cache, longer, inplace=True)
+        assert torch.equal(mk.kv4_attention_decode(q, s.cache, longer), out)
+    assert (out[1] == 1).all() and not out.requires_grad
+
+
+@pytest.mark.gpu
 def test_calls_on_the_gpu_refuse_wrong_arguments(cuda_device):
     s = Server(cuda_device, torch.bfloat16, 128, 2, 16, [20, 3])
     k = torch.zeros(2, 1, 2, 128, dtype=torch.bfloat16, device=cuda_device)
