@@ -8,9 +8,11 @@
 // n 2^-20, so a 32-bit word of eight codes becomes four operand registers with four masks and one shift.  The factor 16 of every
 // second register goes into q (keys) or into the result (values).
 //   * q is scaled by a power of two so that its largest channel is in [2^14, 2^15): exact for bf16 and f16 values.
-//   * Weights times scales are kept in units of the largest scale's power of two so far, so that f16 holds them whatever the size of the
-//     values, and in two halves (hi + lo, 22 bits): a rounded weight's error would be multiplied by a code of 0 .. 15 where the value
-//     itself, with its zero point, may be near zero.  (One half: 6 us of 78 less at 48 long rows, and an error of 2^-11 of the codes' size.)
+//   * Weights times scales are formed in fp32 and brought into f16's range by a power of two for each group of channels and each column, chosen
+//     by the largest such product so far: not by the largest scale, which may be that of a token without weight, of another group, or of a token
+//     that this query does not see.  They are held in two halves (hi + lo, 22 bits, and down to 2^-34 of the largest): a rounded weight's error would be
+//     multiplied by a code of 0 .. 15 where the value itself, with its zero point, may be near zero.  (One half: 6 us of 78 less at 48 long
+//     rows, and an error of 2^-11 of the codes' size.)
 //   * fp32 splits its queries the same way, takes codes less 8, and adds up short chains of products in fp32 (its error against 64 bits
 //     is 2e-7 to 5e-7 of the output, that of sums in fp32 throughout 2e-7 to 9e-7).
 //
@@ -128,16 +130,7 @@ template <typename T>
 struct KaPair;
 template <>
 struct KaPair<__nv_bfloat16> {
-    static constexpr unsigned kExponent = 0x7f80u, kTop = 255u;
-    static constexpr int kShift = 7, kLeast = 23, kBias = 127;
-    // scales as f16, 2^(unit - bias) as 2: a shift of the exponents that makes 2^7 of it, then a product, which makes subnormals where they
-    // are due.  Scales 2^21 times smaller than that become 0.
-    static __device__ __forceinline__ unsigned scales(unsigned w, int unit) {
-        const unsigned c = (unsigned)(unit - 22) * 0x00800080u;
-        const unsigned h = __vmaxu2(w, c) * 8u - c * 8u, f = 0x24002400u;  // 2^-6, twice
-        const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&f));
-        return *reinterpret_cast<const unsigned*>(&r);
-    }
+    static constexpr unsigned kExponent = 0x7f80u;
     static __device__ __forceinline__ unsigned pack(float x, float y) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         return *reinterpret_cast<const unsigned*>(&h);
@@ -146,13 +139,7 @@ struct KaPair<__nv_bfloat16> {
 };
 template <>
 struct KaPair<__half> {
-    static constexpr unsigned kExponent = 0x7c00u, kTop = 31u;
-    static constexpr int kShift = 10, kLeast = 7, kBias = 15;
-    static __device__ __forceinline__ unsigned scales(unsigned w, int unit) {
-        const unsigned f = (unsigned)(16 - unit + 15) * 0x04000400u;  // 2^(16 - unit), twice
-        const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&f));
-        return *reinterpret_cast<const unsigned*>(&h);
-    }
+    static constexpr unsigned kExponent = 0x7c00u;
     static __device__ __forceinline__ unsigned pack(float x, float y) { return pack_half(x, y); }
     static __device__ __forceinline__ float2 unpack(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 };
@@ -173,6 +160,9 @@ __device__ __forceinline__ unsigned as_word(__half2 h) { return *reinterpret_cas
 
 // 2^e, e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// e of a positive number in [2^e, 2^(e + 1))
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
 
 // 2^e <= most < 2^(e + 1), within what pow2 takes on either side
 __device__ __forceinline__ int ka_exponent(float most) { return min(max((int)(__float_as_uint(most) >> 23), 14), 254) - 127; }
@@ -196,11 +186,22 @@ __device__ __forceinline__ void lds_words(const unsigned char* p, unsigned (&w)[
 // Which halves of a pair of tokens t, t + 1 lie below `end`.
 __device__ __forceinline__ unsigned ka_keep(int t, int end) { return (t < end ? 0x0000ffffu : 0u) | (t + 1 < end ? 0xffff0000u : 0u); }
 
-// Weights (two halves) times scales, again in two halves: the product rounded, and what the rounding left plus the weights' second halves.
-__device__ __forceinline__ void ka_weigh(unsigned ph, unsigned pl, unsigned scale, unsigned& hi, unsigned& lo) {
-    const __half2 h = __hmul2(as_half2(ph), as_half2(scale));
-    hi = as_word(h);
-    lo = as_word(__hfma2(as_half2(pl), as_half2(scale), __hfma2(as_half2(ph), as_half2(scale), __hneg2(h))));
+// Weights are at most 2^(kLift + kLag).  f16 has them in two halves, for the zero points, and needs room below; the others hold them as fp32 and
+// as two bf16, and need room above: with weights of at most 1 no sum is larger than the values are.
+template <typename T>
+constexpr int kLift = std::is_same<T, __half>::value ? 7 : -4;
+constexpr int kLag = 4;
+// Weights times scales of a group: the largest one is brought to 2^9 .. 2^10 and may grow to 2^15 before that is done again, by a power of two of
+// at most 2^(120 - kLift - kLag), so that its product with a weight is finite.
+constexpr int kAim = 9;
+template <typename T>
+constexpr int kMostUp = 120 - kLift<T> - kLag;
+
+// A group's scale out of its word of the two-byte types' parameters.
+template <typename T>
+__device__ __forceinline__ float ka_scale(unsigned w) {
+    if constexpr (std::is_same<T, __half>::value) return __low2float(as_half2(w));
+    else return __uint_as_float(w << 16);
 }
 
 // fp32 takes codes less 8 as whole numbers in f16 (`times`: 1, or 16 for the upper half bytes).  Sums of them are no larger than they need to
@@ -208,18 +209,6 @@ __device__ __forceinline__ void ka_weigh(unsigned ph, unsigned pl, unsigned scal
 __device__ __forceinline__ unsigned ka_centred(unsigned code, int times) {
     const unsigned c = times == 1 ? 0x64086408u : 0x64806480u;  // 1024 + 8, 1024 + 128
     return as_word(__hsub2(as_half2(code | 0x64006400u), as_half2(c)));
-}
-
-// The least unit, and what a sum in units of it is multiplied by.
-template <typename T>
-__device__ __forceinline__ int ka_least_unit() {
-    if constexpr (sizeof(T) == 4) return 8;
-    else return KaPair<T>::kLeast;
-}
-template <typename T>
-__device__ __forceinline__ float ka_unit_value(int unit) {
-    if constexpr (sizeof(T) == 4) return pow2(unit - 134);
-    else return pow2(unit - KaPair<T>::kBias - 1);
 }
 
 // Scales and zero points of a token's groups.
@@ -438,7 +427,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
         {
             float q[16];
             const int column = block * 8 + g, token = fdiv(column, p.fd_group);
-            own_limit = length - p.tokens + 1 + token;
+            own_limit = min(length, length - p.tokens + 1 + token);
             float f[2][8], most = 0.f;
             unpack8(q_raw[0], f[0]);
             unpack8(q_raw[1], f[1]);
@@ -507,23 +496,44 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 q_zero[1] = std::is_same<T, __half>::value ? 0u : (second ? part[3] : part[2]);
             }
         }
-        int sees_all = min(length, min(limit[0], limit[1]));  // every column sees the positions below this
+        int sees_all = min(limit[0], limit[1]);  // every column sees the positions below this
         sees_all = min(sees_all, __shfl_xor_sync(kFullMask, sees_all, 1));
         sees_all = min(sees_all, __shfl_xor_sync(kFullMask, sees_all, 2));
 
         // zero_sum: the zero points' part, of column g for every group (fp32), or as an MMA leaves it: row g % 4 (the group), columns 2 j, 2 j + 1
         constexpr int Z = kWide ? G : 4;
-        float o[G][4][4], zero_sum[Z], top = -INFINITY, limit_top = -INFINITY, shift = 0.f, weight_sum = 0.f;
+        // top: what weights are relative to, a whole number of log 2 units no less than the maximum less kLag; shift: kLift - top.  up: the power of
+        // two of weights times scales, of column g
+        float o[G][4][4], zero_sum[Z], up[G], top = -INFINITY, shift = 0.f, weight_sum = 0.f;
 #pragma unroll
         for (int i = 0; i < Z; ++i) zero_sum[i] = 0.f;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr)
+        for (int gr = 0; gr < G; ++gr) {
+            up[gr] = pow2(kMostUp<T>);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[gr][m][i] = 0.f;
-        int unit = ka_least_unit<T>(), unit_limit = -1;  // exponent field of the scale that the values' sums are in units of; none yet
+        }
+        // Brings the sums of the codes down by 2^-by[group], of column g each.
+        auto bring_down = [&](const int (&by)[G]) {
+            bool some = false;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) some |= by[gr] != 0;
+            if (!__any_sync(kFullMask, some)) return;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                const float f = pow2(-min(by[gr], 126));
+                const float c0 = __shfl_sync(kFullMask, f, 8 * j), c1 = __shfl_sync(kFullMask, f, 8 * j + 4);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    o[gr][m][0] *= c0, o[gr][m][1] *= c1;
+                    o[gr][m][2] *= c0, o[gr][m][3] *= c1;
+                }
+            }
+        };
 
+        bool fresh = true;  // no tile has been summed yet
         for (; at < segment_end; at += kKaWarps) {
             if (!dead && !mbar_wait(&bars[stage], use & 1, &s_abort)) dead = true;
             dead = __any_sync(kFullMask, dead);
@@ -603,125 +613,104 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             transpose8(s[0], s[1]);
             transpose8(s[2], s[3]);
 
-            // ---- scales of the values of the lane's four tokens.  The sums are kept in units of a scale's power of two, so that f16 holds
-            // weights times scales, and the unit is raised when a scale is 2^4 times larger.  The exponents' bits or'ed
-            // together are no smaller than the largest; only where that says so, it is looked for.
-            unsigned sw[2][G];  // two-byte types: pairs of tokens
-            float vs[4][kWide ? G : 1], vz[4][kWide ? G : 1];
-            bool larger;
-            if constexpr (!kWide) {
-                unsigned w[4][G], bits = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) lds_words(v_params + (2 * j + (i & 1) + 8 * (i >> 1)) * (G * 4), w[i]);
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) sw[0][gr] = __byte_perm(w[0][gr], w[1][gr], 0x5410), sw[1][gr] = __byte_perm(w[2][gr], w[3][gr], 0x5410);
-                if (edge) {  // behind the row's end anything may lie
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const unsigned keep = ka_keep(first + 2 * j + 8 * x, length);
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) sw[x][gr] &= keep;
-                    }
-                }
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) bits |= sw[0][gr] | sw[1][gr];
-                larger = (int)((bits | bits >> 16) & KaPair<T>::kExponent) > unit_limit * (1 << KaPair<T>::kShift);
-            } else {
-                unsigned bits = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = 2 * j + (i & 1) + 8 * (i >> 1);
-                    load_params<T, G>(v_params + t * (G * 8), vs[i], vz[i]);
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        if (edge && first + t >= length) vs[i][gr] = vz[i][gr] = 0.f;
-                        bits |= __float_as_uint(vs[i][gr]);
-                    }
-                }
-                larger = (int)(bits >> 23) > unit_limit;
-            }
-
-            // ---- maximum.  Weights are taken relative to `top`, which follows the maximum only when that is 2^4 times larger: then, and not
-            // with every tile, what has been summed is brought to the new one.
-            bool poisoned = false;
+            // ---- maximum.  `top` follows it only when it is 2^kLag times larger: then, and not with every tile, what has been summed is brought
+            // to the new one.
             float most = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-            if (__any_sync(kFullMask, larger || most > limit_top)) {
-                float down = 1.f;
-                if (__any_sync(kFullMask, larger)) {
-                    int largest = 0;  // an exponent field; that of a NaN is no size: other columns may not see it
-                    if constexpr (!kWide) {
-#pragma unroll
-                        for (int i = 0; i < 4 * G; ++i) {
-                            const unsigned f = (sw[i / 2 / G][i / 2 % G] >> (16 * (i & 1)) & KaPair<T>::kExponent) >> KaPair<T>::kShift;
-                            if (f == KaPair<T>::kTop) poisoned = true;
-                            else largest = max(largest, (int)f);
-                        }
-                        poisoned = __any_sync(kFullMask, poisoned);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int gr = 0; gr < G; ++gr) {
-                                const int f = (int)(__float_as_uint(vs[i][gr]) >> 23);
-                                if (f < 255) largest = max(largest, min(f, 253));
-                            }
-                    }
-                    largest = __reduce_max_sync(kFullMask, largest);
-                    if (largest > unit) {
-                        down = pow2(max(unit - largest, -126));
-                        unit = largest;
-                    }
-                    unit_limit = min(unit + 3, 254);  // the exponent of a NaN is always beyond it
-                }
-                const float m = fmaxf(top, most);
-                const float corr = m == -INFINITY ? 0.f : exp2f((top - m) * mult);  // nothing has been summed without a maximum
-                top = m;
-                limit_top = m == -INFINITY ? m : m + 4.f / mult;
-                shift = m == -INFINITY ? 0.f : 6.f - m * mult;
+            if (__any_sync(kFullMask, fmaf(most, mult, -(float)kLag) > top)) {
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
+                const float next = fmaxf(top, ceilf(most * mult)), next_shift = next == -INFINITY ? 0.f : kLift<T> - next;
+                const float drop = top == -INFINITY ? 0.f : shift - next_shift, corr = exp2f(-drop);  // nothing has been summed without a maximum
+                top = next, shift = next_shift;
                 weight_sum *= corr;
-                const float k0 = __shfl_sync(kFullMask, corr, 8 * j), k1 = __shfl_sync(kFullMask, corr, 8 * j + 4);
-                const float c0 = k0 * down, c1 = k1 * down;
                 if constexpr (kWide) {
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) zero_sum[gr] *= corr;
                 } else {
-                    zero_sum[0] *= k0, zero_sum[1] *= k1;
+                    zero_sum[0] *= __shfl_sync(kFullMask, corr, 8 * j), zero_sum[1] *= __shfl_sync(kFullMask, corr, 8 * j + 4);
                 }
+                // weights get smaller, `up` grows by as much, and the sums stay as they are; at its end they get smaller
+                const int by = (int)fminf(drop, 1000.f);
+                int rest[G];
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) {
-                        o[gr][m][0] *= c0, o[gr][m][1] *= c1;
-                        o[gr][m][2] *= c0, o[gr][m][3] *= c1;
-                    }
+                for (int gr = 0; gr < G; ++gr) {
+                    const int e = exponent_of(up[gr]), n = min(e + by, kMostUp<T>);
+                    up[gr] = pow2(n);
+                    rest[gr] = e + by - n;
+                }
+                bring_down(rest);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = kWide ? exp2f(fmaf(s[i], mult, shift)) : exp2_approx(fmaf(s[i], mult, shift));
+            weight_sum += (s[0] + s[1]) + (s[2] + s[3]);
 
-            // Weights, 2^6 times as large for the two-byte types (at most 2^10, and 2^5 for a scale, so that a product stays below 2^16): f16
-            // then holds those down to 2^-31 of the largest.  Many that small can be all there is, where the value of a key that draws
-            // nearly everything is 0.  fp32: the difference first, which is exact where it matters, and 2^7 goes into `shrink`.
+            // ---- scales of the values of the lane's four tokens; what the column does not see may be anything, a NaN too
+            unsigned vw[4][kWide ? 1 : G];
+            float vs[4][kWide ? G : 1], vz[4][kWide ? G : 1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s[i] = kWide ? exp2f((s[i] - (top == -INFINITY ? 0.f : top)) * mult) : exp2_approx(fmaf(s[i], mult, shift));
-
-            // ---- weights times scales, in two halves; the zero points' part
-            unsigned hi[G][2], lo[G][2];
-            if constexpr (!kWide) {
-                unsigned scale[2][G];
+            for (int i = 0; i < 4; ++i) {
+                const int t = 2 * j + (i & 1) + 8 * (i >> 1);
+                if constexpr (kWide) load_params<T, G>(v_params + t * (G * 8), vs[i], vz[i]);
+                else lds_words(v_params + t * (G * 4), vw[i]);
+            }
+            if (edge) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) scale[x][gr] = KaPair<T>::scales(sw[x][gr], unit);
-                if (std::is_same<T, __nv_bfloat16>::value && poisoned) {  // the shift of exponents does not do for a NaN
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
+                for (int i = 0; i < 4; ++i)
+                    if (first + 2 * j + (i & 1) + 8 * (i >> 1) >= own_limit) {
 #pragma unroll
                         for (int gr = 0; gr < G; ++gr) {
-                            const float2 f = KaPair<T>::unpack(sw[x][gr]);
-                            scale[x][gr] = pack_half(f.x * pow2(128 - unit), f.y * pow2(128 - unit));
+                            if constexpr (kWide) vs[i][gr] = vz[i][gr] = 0.f;
+                            else vw[i][gr] = 0u;
                         }
+                    }
+            }
+            auto scale_of = [&](int i, int gr) {
+                if constexpr (kWide) return vs[i][gr];
+                else return ka_scale<T>(vw[i][gr]);
+            };
+
+            // ---- weights times scales, in two halves.  They are what has to lie in f16's range, whatever weights and scales are by themselves: in
+            // units of their own for each group and column.  Where one goes beyond, the units are chosen again.
+            unsigned hi[G][2], lo[G][2];
+#pragma unroll 1
+            for (int turn = 0;; ++turn) {
+                __half2 largest = __float2half2_rn(0.f);
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const f32x2 weights = mul_pair(pair_of(s[2 * x], s[2 * x + 1]), pair_of(up[gr], up[gr]));
+                        const f32x2 both = mul_pair(weights, pair_of(scale_of(2 * x, gr), scale_of(2 * x + 1, gr)));
+                        split_half(first_of(both), second_of(both), hi[gr][x], lo[gr][x]);
+                        largest = __hmax2(largest, __habs2(as_half2(hi[gr][x])));
+                    }
                 }
+                const bool fits = __hbleu2(largest, __float2half2_rn(32768.f));
+                if (turn == 1 || __all_sync(kFullMask, fits)) break;
+                int by[G];
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    float m = 0.f;  // 2^-20 of the largest, which is finite
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(s[i] * 0x1p-20f * scale_of(i, gr)));
+                    m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 2));
+                    const int e = exponent_of(up[gr]), size = exponent_of(m) + 20;
+                    const int n = m == 0.f ? e : max(min(e, kAim - size), -126);
+                    up[gr] = pow2(n);
+                    by[gr] = e - n;
+                }
+                if (!fresh) bring_down(by);
+            }
+            fresh = false;
+
+            // ---- the zero points' part
+            if constexpr (kWide) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) zero_sum[gr] = fmaf(s[i], fmaf(8.f, vs[i][gr], vz[i][gr]), zero_sum[gr]);
+            } else {
                 unsigned z[4], za[2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) z[i] = *reinterpret_cast<const unsigned*>(v_params + ((2 * j + (i & 1) + 8 * (i >> 1)) * G + g % G) * 4);
@@ -735,55 +724,19 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                         za[x] &= keep;
                     }
                 }
-                weight_sum += (s[0] + s[1]) + (s[2] + s[3]);
-                unsigned ph[2], pl[2];
-                split_half(s[0], s[1], ph[0], pl[0]);
-                split_half(s[2], s[3], ph[1], pl[1]);
-                if (std::is_same<T, __nv_bfloat16>::value) {  // operands of one type: the weights once more, as two bf16 (16 bits)
-                    unsigned bh[2], bl[2];
+                unsigned ph[2], pl[2];  // operands of one type: two halves of f16 (22 bits) or two of bf16 (16 bits)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        bh[x] = KaPair<__nv_bfloat16>::pack(s[2 * x], s[2 * x + 1]);
-                        const float2 f = KaPair<__nv_bfloat16>::unpack(bh[x]);
-                        bl[x] = KaPair<__nv_bfloat16>::pack(s[2 * x] - f.x, s[2 * x + 1] - f.y);
+                for (int x = 0; x < 2; ++x) {
+                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                        ph[x] = KaPair<T>::pack(s[2 * x], s[2 * x + 1]);
+                        const float2 f = KaPair<T>::unpack(ph[x]);
+                        pl[x] = KaPair<T>::pack(s[2 * x] - f.x, s[2 * x + 1] - f.y);
+                    } else {
+                        split_half(s[2 * x], s[2 * x + 1], ph[x], pl[x]);
                     }
-                    ka_mma_params<T>(zero_sum, za[0], 0u, za[1], 0u, bl[0], bl[1]);
-                    ka_mma_params<T>(zero_sum, za[0], 0u, za[1], 0u, bh[0], bh[1]);
-                } else {
-                    ka_mma_params<T>(zero_sum, za[0], 0u, za[1], 0u, pl[0], pl[1]);
-                    ka_mma_params<T>(zero_sum, za[0], 0u, za[1], 0u, ph[0], ph[1]);
                 }
-                if (edge) {  // what the column does not see may be a NaN
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const unsigned keep = ka_keep(first + 2 * j + 8 * x, own_limit);
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr] & keep, hi[gr][x], lo[gr][x]);
-                    }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) ka_weigh(ph[x], pl[x], scale[x][gr], hi[gr][x], lo[gr][x]);
-                }
-            } else {
-                const float shrink = pow2(134 - unit);
-                weight_sum += (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (edge && first + 2 * j + (i & 1) + 8 * (i >> 1) >= own_limit) {
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) vs[i][gr] = vz[i][gr] = 0.f;
-                    }
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) zero_sum[gr] = fmaf(s[i], fmaf(8.f, vs[i][gr], vz[i][gr]), zero_sum[gr]);
-                    s[i] *= shrink;
-                }
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) {
-                    split_half(s[0] * vs[0][gr], s[1] * vs[1][gr], hi[gr][0], lo[gr][0]);
-                    split_half(s[2] * vs[2][gr], s[3] * vs[3][gr], hi[gr][1], lo[gr][1]);
-                }
+                ka_mma_params<T>(zero_sum, za[0], 0u, za[1], 0u, pl[0], pl[1]);
+                ka_mma_params<T>(zero_sum, za[0], 0u, za[1], 0u, ph[0], ph[1]);
             }
 
             // ---- values
@@ -847,11 +800,10 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
         }
         if (j == 0) {
             const int c = warp * 8 + g;
-            s_max[c] = top * mult;
+            s_max[c] = top == -INFINITY ? top : -shift;
             s_sum[c] = weight_sum;
         }
         __syncthreads();
-        const float grow = ka_unit_value<T>(unit);
         const long long slot = 2ll * blockIdx.x + (segment > begin ? 1 : 0);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {  // the columns 2 j + c of all warps; a warp then adds one of them up
@@ -863,11 +815,12 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             // channel 8 g + i of a group at 8 i + g
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
+                const float back = __uint_as_float(0x7f000000u - __float_as_uint(__shfl_sync(kFullMask, up[gr], (2 * j + c) * 4)));  // 1 / up
                 const float zero = kWide ? __shfl_sync(kFullMask, zero_sum[gr % Z], (2 * j + c) * 4) : __shfl_sync(kFullMask, zero_sum[c], gr * 4 + j);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int m4 = (k >> 2) * 2 + (k & 1), half = (k >> 1) & 1;  // channel 8 g + k lies in these registers
-                    const float sum = fmaf(o[gr][m4][2 * half + c] * ((m4 & 1 ? 0.0625f : 1.f) * (kWide ? 1.f : 0x1p24f)), grow, zero);
+                    const float sum = fmaf(o[gr][m4][2 * half + c] * ((m4 & 1 ? 0.0625f : 1.f) * (kWide ? 1.f : 0x1p24f)), back, zero);
                     s_fold[(warp * 4 + j) * C::kFoldRow + gr * kKv4Group + k * 8 + g] = sum * weight;
                 }
             }

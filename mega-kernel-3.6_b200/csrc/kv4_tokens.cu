@@ -139,15 +139,6 @@ __device__ __forceinline__ unsigned codes_exact(const float (&x)[8], float zero,
     return four_exact(make_float4(x[0], x[1], x[2], x[3]), zero, scale) | four_exact(make_float4(x[4], x[5], x[6], x[7]), zero, scale) << 16;
 }
 
-// Two fp32 operations an instruction, each rounded as one alone would be.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair_of(float x, float y) {
-    f32x2 d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-    return d;
-}
-__device__ __forceinline__ float first_of(f32x2 v) { return __uint_as_float((unsigned)v); }
-__device__ __forceinline__ float second_of(f32x2 v) { return __uint_as_float((unsigned)(v >> 32)); }
 __device__ __forceinline__ f32x2 add_pair(f32x2 a, f32x2 b) {
     f32x2 d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));

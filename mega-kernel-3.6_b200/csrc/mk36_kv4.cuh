@@ -90,6 +90,21 @@ __device__ __forceinline__ void kv4_unpack(const Kv4Param<float>& p, float& scal
     zero = p.zero;
 }
 
+// Two fp32 operations an instruction, each rounded as one alone would be.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float x, float y) {
+    f32x2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ float first_of(f32x2 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float second_of(f32x2 v) { return __uint_as_float((unsigned)(v >> 32)); }
+__device__ __forceinline__ f32x2 mul_pair(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 #endif  // __CUDACC__
 
 }  // namespace mk36

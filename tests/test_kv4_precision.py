@@ -1,0 +1,175 @@
+"""Accuracy of attention over the 4-bit paged cache, by group of 64 channels and by what the softmax lets through: values of very different
+sizes in one row, in one head, and behind what a query sees."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import mega_kernel_qwen36 as mk
+from oracle import kv4_oracle as oracle
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _parameters(pool, pages, length, head, d, dtype):
+    """Scales and zero points of a row's values, ``[length, d / 64]`` each in 64 bits."""
+    page_size = pool.shape[2] * oracle.TILE
+    tiles = np.stack([pool[pages[i * oracle.TILE // page_size], head, i % (page_size // oracle.TILE)] for i in range(-(-length // oracle.TILE))])
+    first = 16 * d + d * dtype.itemsize // 2
+    param = torch.from_numpy(tiles[:, first : first + d * dtype.itemsize // 2].copy()).view(dtype).double().reshape(-1, d // oracle.GROUP, 2)[:length]
+    return param[..., 0], param[..., 1]
+
+
+class Row:
+    """Rows of one KV head whose scores are exact: the keys' first group has the entries 0 to 15 (scale 1, zero point 0) and a
+    query is one channel of it, so a score is one product of a query's channel and a code.  ``copies``: so many rows hold each
+    row's pages, enough of them that a warp works through several tiles in turn."""
+
+    def __init__(self, dev, dtype, d, lengths, page_size=32, copies=1):
+        self.dev, self.dtype, self.d, self.lengths, self.copies = dev, dtype, d, list(lengths), copies
+        per = [-(-n // page_size) for n in lengths]
+        total, width = sum(per), max(per) + 1
+        self.table, at = [], 0
+        for n in per:
+            self.table.append(list(range(at + n - 1, at - 1, -1)) + [-1] * (width - n))
+            at += n
+        self.pool = np.zeros((total, 1, page_size // 16, oracle.tile_bytes(d, dtype)), np.uint8)
+
+    def fill(self, codes, v):
+        """codes: of the channel that queries look at, 0 to 14, for all tokens of all rows; v ``[tokens, d]``."""
+        k = torch.zeros(len(codes), 1, self.d)
+        k[:, 0, 0], k[:, 0, 1] = torch.tensor(codes, dtype=torch.float32), 15
+        self.codes = codes
+        oracle.append(self.pool, self.table, self.lengths, k.to(self.dtype), v[:, None].to(self.dtype), self.lengths)
+        on = lambda x: torch.tensor(x, dtype=torch.int32, device=self.dev)
+        self.cache = mk.Kv4Cache(torch.from_numpy(self.pool).to(self.dev), self.d, self.dtype)
+        each = lambda x: on(x).repeat_interleave(self.copies, 0)
+        self.gpu = mk.PageTable(each(self.table), each(self.lengths), torch.full((len(self.pool),), self.copies, dtype=torch.int32, device=self.dev))
+
+    def queries(self, step, tokens=1, heads=4):
+        """Queries whose score grows by `step` (a number of few bits) with each code; the scale of the call is 1."""
+        q = torch.zeros(len(self.lengths) * self.copies, tokens, heads, self.d)
+        q[..., 0] = step
+        return q.to(self.dtype)
+
+    def check(self, q, out, step):
+        """Limits are for each group by itself, from what the softmax leaves of its entries.  With exact scores a weight is off by the
+        roundings of the factor to log 2 units (three of 2^-24 of the score's distance to the largest), of the difference, of the
+        exponential (2^-22) and of its products with scale and unit (2^-24 each, 2^-22 in two halves): 2^-21 of itself and of the
+        distance; zero points of bf16 meet weights of two bf16 (2^-16).  Sums: at most 2^-22 of what they hold for each tile of 16 that
+        a running sum takes and for each of a few joins.  The same for the denominator.  A weight of f16 that meets a
+        zero point is held down to 2^-31 of the largest, a weight times scale down to 2^-34 of the group's largest."""
+        tokens, at, worst = q.shape[1], 0, 0.0
+        out = out.cpu().double().view(q.shape)
+        for r, n in enumerate(self.lengths):
+            codes = torch.tensor(self.codes[at : at + n], dtype=torch.float64)
+            at += n
+            _, values = oracle.row_entries(self.pool, self.table[r], n, 0, self.d, self.dtype)
+            scale, zero = _parameters(self.pool, self.table[r], n, 0, self.d, self.dtype)
+            for i in range(tokens):
+                seen = n - tokens + i + 1
+                score = codes[:seen] * step
+                weight = torch.softmax(score, 0)
+                want = weight @ values[:seen]
+                share = 2 * (((score.max() - score)[:, None] + 1) * 2.0**-21 + 2.0**-20 + (n / 16 + 8) * 2.0**-22)
+                size = zero[:seen].abs() + 15 * scale[:seen].abs()
+                limit = (weight[:, None] * size * share).sum(0) + seen * 2.0**-34 * 15 * (weight[:, None] * scale[:seen]).amax(0)
+                if self.dtype is torch.bfloat16:
+                    limit += 2.0**-16 * (weight[:, None] * zero[:seen].abs()).sum(0)
+                if self.dtype is torch.float16:
+                    limit += (torch.minimum(weight, 2.0**-31 * weight.max())[:, None] * zero[:seen].abs()).sum(0)
+                limit = limit.repeat_interleave(oracle.GROUP) + want.abs() * torch.finfo(self.dtype).eps / 2 * 1.01
+                limit += torch.finfo(self.dtype).smallest_normal * torch.finfo(self.dtype).eps / 2 * 1.01  # half a step of the smallest numbers
+                off = (out[r * self.copies : (r + 1) * self.copies, i] - want).abs() / limit
+                worst = max(worst, off.max().item())
+        assert worst <= 1, f"off by {worst:.3g} of the limit"
+
+
+def _sizes(dtype):
+    """Factors between sizes of values that the type can hold, with ordinary values on one side."""
+    return [2.0**e for e in ((8, 16, 20) if dtype is torch.float16 else (8, 12, 16, 20, 24, 60))]
+
+
+def _base(dtype, factor):
+    """Size of the smaller values: in f16 the larger ones have to stay below 65504."""
+    return 4096.0 / factor if dtype is torch.float16 else 1.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,copies", [(64, 1), (128, 1), (256, 1), (64, 200), (128, 200), (256, 200)])
+def test_a_token_that_no_query_heeds_may_have_values_of_any_size(cuda_device, dtype, d, copies):
+    step = 4.25  # scores of 0 to 59.5: the loud tokens' weights are 2^-86 of the others'
+    for factor in _sizes(dtype):
+        row = Row(cuda_device, dtype, d, [16, 100, 700], copies=copies)
+        gen = torch.Generator().manual_seed(7)
+        v = torch.randn(816, d, generator=gen) * _base(dtype, factor)
+        codes = [14] * 816
+        for loud in (3, 16, 16 + 99, 116 + 350, 116 + 351, 815):  # first, middle and last tokens of a row
+            codes[loud] = 0
+            v[loud] *= factor
+        row.fill(codes, v)
+        q = row.queries(step)
+        row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0), step)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [128, 256])
+def test_groups_of_a_head_may_have_values_of_any_size(cuda_device, dtype, d):
+    for factor in _sizes(dtype):
+        row = Row(cuda_device, dtype, d, [37, 300])
+        gen = torch.Generator().manual_seed(8)
+        v = torch.randn(337, d, generator=gen) * _base(dtype, factor)
+        v[:, 64:128] *= factor
+        row.fill(torch.randint(8, 15, (337,), generator=gen).tolist(), v)
+        q = row.queries(0.5)
+        row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0), 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("order", ["within a tile", "rising", "falling"])
+def test_values_that_shrink_as_the_scores_grow(cuda_device, dtype, d, order):
+    """Weight times value is of one size throughout, though weights and values each go over many powers of two."""
+    n = 15 * 16
+    step = 1.5 if dtype is torch.float16 else 5.5  # over all codes 2^-30, 2^-111
+    codes = [i % 15 if order == "within a tile" else i // 16 if order == "rising" else 14 - i // 16 for i in range(n)]
+    row = Row(cuda_device, dtype, d, [n], copies=1000)
+    size = torch.exp(-step * torch.tensor(codes, dtype=torch.float64)) * (30000 if dtype is torch.float16 else 1e15)
+    row.fill(codes, (torch.randn(n, d, generator=torch.Generator().manual_seed(9)).double().clamp(-2, 2) * size[:, None]).float())
+    q = row.queries(step)
+    row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0), step)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [1, 4])
+def test_later_tokens_of_a_draft_do_not_change_earlier_queries(cuda_device, dtype, heads):
+    for factor in _sizes(dtype):
+        row = Row(cuda_device, dtype, 64, [70, 37, 16])
+        gen = torch.Generator().manual_seed(10)
+        v = torch.randn(123, 64, generator=gen) * _base(dtype, factor)
+        for last in (69, 106, 122):
+            v[last] *= factor
+        row.fill(torch.randint(8, 15, (123,), generator=gen).tolist(), v)
+        q = row.queries(0.5, tokens=4, heads=heads)
+        out = mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0)
+        row.check(q, out, 0.5)
+        # a call that ends before the loud token
+        early = mk.kv4_attention_decode(q[:, :3].contiguous().to(cuda_device), row.cache, mk.PageTable(row.gpu.pages, row.gpu.lengths - 1, row.gpu.refcounts), scale=1.0)
+        assert torch.allclose(out[:, :3].double(), early.double(), rtol=2 * torch.finfo(dtype).eps, atol=_base(dtype, factor) * 2.0**-14)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_values_near_the_largest_numbers_and_the_smallest(cuda_device, dtype):
+    gen = torch.Generator().manual_seed(11)
+    for size in (torch.finfo(dtype).max / 64, 2.0**-100, torch.finfo(dtype).smallest_normal * 512):
+        row = Row(cuda_device, dtype, 64, [50, 1])
+        row.fill([14] * 51, (torch.randn(51, 64, generator=gen).clamp(-3, 3) / 3).double().mul(size).float())
+        q = row.queries(0.5)
+        row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0), 0.5)
