@@ -390,7 +390,6 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
     };
     const unsigned char *src_now = look_up(), *src_next = nullptr;
     int requested = 0;
-    unsigned lost = 0;  // bit s: stage s holds another tile, because the table names none
     auto request = [&](int stage) {
         if (begin + warp + requested * kKaWarps >= end) return;
         if (requested % 32 == 0) {
@@ -398,10 +397,16 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             src_next = look_up();
         }
         const unsigned char* src = reinterpret_cast<const unsigned char*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(src_now), requested % 32));
-        lost = (lost & ~(1u << stage)) | (src ? 0u : 1u << stage);
-        if (lane == 0) {
-            mbar_arrive_expect_tx(&bars[stage], C::kTile);
-            bulk_copy_g2s(ring + stage * C::kTile, src ? src : p.cache.pool, C::kTile, &bars[stage]);
+        if (src) {
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&bars[stage], C::kTile);
+                bulk_copy_g2s(ring + stage * C::kTile, src, C::kTile, &bars[stage]);
+            }
+        } else {  // a tile of NaN: it reaches the queries that see it, like any other
+            for (int i = lane; i < C::kTile / 16; i += 32) reinterpret_cast<uint4*>(ring + stage * C::kTile)[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next copy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[stage]);
         }
         ++requested;
     };
@@ -537,8 +542,10 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
         for (; at < segment_end; at += kKaWarps) {
             if (!dead && !mbar_wait(&bars[stage], use & 1, &s_abort)) dead = true;
             dead = __any_sync(kFullMask, dead);
-            if (dead || (lost >> stage & 1u)) weight_sum = __uint_as_float(0x7fc00000u);
-            if (dead) continue;
+            if (dead) {
+                weight_sum = __uint_as_float(0x7fc00000u);
+                continue;
+            }
             const unsigned char *codes = ring + stage * C::kTile, *params = codes + 2 * kv4_code_bytes(D), *v_params = params + kv4_param_bytes(D, sizeof(T));
             const int first = (now.tile + (at - segment)) * kKv4Tile;
 

@@ -173,3 +173,28 @@ def test_values_near_the_largest_numbers_and_the_smallest(cuda_device, dtype):
         row.fill([14] * 51, (torch.randn(51, 64, generator=gen).clamp(-3, 3) / 3).double().mul(size).float())
         q = row.queries(0.5)
         row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0), 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("missing", [-1, 10**6])
+@pytest.mark.parametrize("copies", [1, 300])
+def test_a_missing_page_reaches_the_queries_that_see_it_and_no_other(cuda_device, dtype, missing, copies):
+    row = Row(cuda_device, dtype, 128, [70, 64, 40, 3], page_size=32, copies=copies)
+    gen = torch.Generator().manual_seed(12)
+    row.fill(torch.randint(8, 15, (177,), generator=gen).tolist(), torch.randn(177, 128, generator=gen))
+    q = row.queries(0.5, tokens=9)
+    whole = mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0)
+    pages = row.gpu.pages.clone()
+    pages[:copies, 2] = missing  # positions 64 to 69: the last six queries
+    pages[copies : 2 * copies, 0] = missing  # all of them
+    pages[2 * copies : 3 * copies, 1] = missing  # positions 32 to 39: all but the first query, whose last position is 31
+    pages[3 * copies :, 0] = missing  # the last three; the others see nothing
+    assert row.table[0][2] == 0
+    row.cache.pool[0].fill_(0xFF)  # NaN parameters in a page that nobody holds now, the pool's first
+    out = mk.kv4_attention_decode(q.to(cuda_device), row.cache, mk.PageTable(pages, row.gpu.lengths, row.gpu.refcounts), scale=1.0).unflatten(0, (4, copies))
+    whole = whole.unflatten(0, (4, copies))
+    for r, good in enumerate((3, 0, 1, 6)):
+        assert torch.isnan(out[r, :, good:]).all()
+        assert torch.allclose(out[r, :, :good].double(), whole[r, :, :good].double(), rtol=2 * torch.finfo(dtype).eps, atol=2.0**-14)
+    assert (out[3, :, :6] == 0).all()
