@@ -7,7 +7,9 @@
 // What is left per element is to turn codes into operands, and there f16 helps: the bits 0x000n are the subnormal n 2^-24, 0x00n0 is
 // n 2^-20, so a 32-bit word of eight codes becomes four operand registers with four masks and one shift.  The factor 16 of every
 // second register goes into q (keys) or into the result (values).
-//   * q is scaled by a power of two so that its largest channel is in [2^14, 2^15): exact for bf16 and f16 values.
+//   * q is scaled by a power of two so that its largest channel is in [2^14, 2^15): exact for bf16 and f16 values, but for what lies below steps of
+//     2^-35 of that channel.  A group whose largest channel is smaller than 2^-12 of it has a power of its own (its keys may be as much larger), and
+//     the groups' products are then brought together in fp32.
 //   * Weights times scales are formed in fp32 and brought into f16's range by a power of two for each group of channels and each column, chosen
 //     by the largest such product so far: not by the largest scale, which may be that of a token without weight, of another group, or of a token
 //     that this query does not see.  They are held in two halves (hi + lo, 22 bits, and down to 2^-34 of the largest): a rounded weight's error would be
@@ -71,7 +73,7 @@ struct KaConfig {
     static constexpr int kFoldRow = D + 8;  // the lanes of a store (g, j), rows j apart, fall into 32 banks
     static constexpr int kFold = kKaWarps * 4 * kFoldRow * 4;
     static constexpr int kOperands = kQParts * kGroups * 4 * 32 * 8;  // of the queries
-    static constexpr int kStats = (kKaWarps * 8 * 2 + 8 * kGroups * 2) * 4;
+    static constexpr int kStats = (kKaWarps * 8 * 2 + 8 * kGroups * 3) * 4;
     static constexpr int kRoom = 232448 / kCtas - 1024 - kFold - kOperands - kStats - 512;
     static constexpr int kMost = kRoom / (kKaWarps * kTile);
     static constexpr int kStages = kMost < 8 ? kMost : 8;
@@ -333,7 +335,8 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
     float* s_sum = s_max + kKaWarps * 8;           // [warp][8]
     float* s_most = s_sum + kKaWarps * 8;          // [G][8]: largest |q|
     float* s_qsum = s_most + G * 8;                // [8][G]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(s_qsum + 8 * G) + warp * C::kStages;
+    float* s_qunit = s_qsum + 8 * G;               // [8][G]: unit of a group's products, where they have units of their own
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(s_qunit + 8 * G) + warp * C::kStages;
     if (lane == 0) {
         for (int i = 0; i < C::kStages; ++i) mbar_init(&bars[i], 1);
         mbar_init_fence();
@@ -428,6 +431,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
         float mult;                     // factor of column g's scores, in units of log 2
         float q_sum[2][kWide ? G : 1];  // fp32: sums over the groups' channels of columns 2 j, 2 j + 1
         unsigned q_zero[2];             // two-byte types: the sums of column g as operand registers, against the zero points
+        bool spread = false;            // of a column, groups' largest channels are far apart
         int limit[2], own_limit;        // positions that the columns 2 j, 2 j + 1 see, and column g
         {
             float q[16];
@@ -449,7 +453,13 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) most = fmaxf(most, s_most[gr * 8 + g]);
             if (warp < G) {
-                const float up = copysignf(pow2(14 - ka_exponent(most)), p.scale);  // the scale's sign goes into q
+                const int all = ka_exponent(most);
+                int unit = all;
+                if (G > 1) {
+                    const float own = s_most[warp * 8 + g];
+                    if (own > 0.f && own < 0x1p-12f * most) unit = max(ka_exponent(own), all - 126);
+                }
+                const float up = copysignf(pow2(14 - unit), p.scale);  // the scale's sign goes into q
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -458,7 +468,10 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 }
                 sum += __shfl_xor_sync(kFullMask, sum, 1);
                 sum += __shfl_xor_sync(kFullMask, sum, 2);
-                if (j == 0) s_qsum[g * G + warp] = kWide ? sum : sum * pow2(-24);
+                if (j == 0) {
+                    s_qsum[g * G + warp] = sum * pow2(unit - all) * (kWide ? 1.f : pow2(-24));
+                    if (G > 1) s_qunit[g * G + warp] = pow2(unit - all);
+                }
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {  // MMA m takes the codes 2 (m % 2), + 1, + 4, + 5 of word m / 2
                     const float* x = &q[8 * w];
@@ -474,6 +487,11 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             __syncthreads();
             // not 0, so that a score of -infinity stays one
             mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, (kWide ? 0 : 24) - 14 + ka_exponent(most)), 1e-37f);
+            if (G > 1) {  // in all warps alike: each looks at all columns
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) spread |= s_qunit[g * G + gr] != 1.f;
+                spread = __any_sync(kFullMask, spread);
+            }
             // what belongs to a column, for the lanes that hold it in the products' layout: columns 2 j, 2 j + 1
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -496,6 +514,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                     const float2 f = KaPair<T>::unpack(part[i]);
                     x[0] -= f.x, x[1] -= f.y;
                 }
+                if (spread) part[0] = part[1] = part[2] = part[3] = 0u;  // in fp32 with the products, below
                 const bool second = j >> 1;
                 q_zero[0] = second ? part[1] : part[0];
                 q_zero[1] = std::is_same<T, __half>::value ? 0u : (second ? part[3] : part[2]);
@@ -602,6 +621,16 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                         }
                     }
                 }
+            }
+            if (G > 1 && spread) {
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at_q = (2 * j + (i & 1)) * G + gr;
+                        acc[gr][i] *= s_qunit[at_q];
+                        if constexpr (!kWide) s[i] = fmaf(kz[i >> 1][gr], s_qsum[at_q], s[i]);
+                    }
             }
 #pragma unroll
             for (int gr = 0; gr < G; ++gr)

@@ -9,6 +9,7 @@ import torch
 
 import mega_kernel_qwen36 as mk
 from oracle import kv4_oracle as oracle
+from test_kv4_cache import Server, check_attention
 
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 
@@ -198,3 +199,25 @@ def test_a_missing_page_reaches_the_queries_that_see_it_and_no_other(cuda_device
         assert torch.isnan(out[r, :, good:]).all()
         assert torch.allclose(out[r, :, :good].double(), whole[r, :, :good].double(), rtol=2 * torch.finfo(dtype).eps, atol=2.0**-14)
     assert (out[3, :, :6] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,hq,tokens", [(128, 8, 1), (256, 3, 1), (128, 2, 5)])
+def test_groups_of_a_query_may_be_of_any_size(cuda_device, dtype, d, hq, tokens):
+    """One group of the keys is large where the queries are small, and another the other way round, so that both count in the scores."""
+    for a in (3, 8, 12, 13) if dtype is torch.float16 else (4, 10, 15, 30, 50):
+        s = Server(cuda_device, dtype, d, 1, 32, [90, 17])
+        gen = torch.Generator().manual_seed(a)
+        k, v = (torch.randn(107, 1, d, generator=gen).clamp(-3, 3) for _ in range(2))
+        q = torch.randn(2, tokens, hq, d, generator=gen).clamp(-3, 3)
+        k[..., :64], q[..., :64] = k[..., :64] * 2.0**-a, q[..., :64] * 2.0**a
+        k[..., 64:128], q[..., 64:128] = k[..., 64:128] * 2.0**a, q[..., 64:128] * 2.0**-a
+        k[..., 128:] = 0
+        if hq > 2:
+            q[1, :, 1, 64:] = 0  # and one whose other groups are nothing
+        oracle.append(s.pool, s.table, s.lengths, k.to(dtype), v.to(dtype), s.lengths)
+        s.cache.pool.copy_(torch.from_numpy(s.pool))
+        q = q.to(dtype)
+        for scale in (0.2, -0.2):
+            check_attention(s, q, mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu, scale=scale), scale)
