@@ -193,6 +193,7 @@ __device__ __forceinline__ unsigned ka_keep(int t, int end) { return (t < end ? 
 template <typename T>
 constexpr int kLift = std::is_same<T, __half>::value ? 7 : -4;
 constexpr int kLag = 4;
+constexpr int kMostQ = 100;  // queries larger than 2^100 have products in units of 2^100: the factor to log 2 units stays finite
 // Weights times scales of a group: the largest one is brought to 2^9 .. 2^10 and may grow to 2^15 before that is done again, by a power of two of
 // at most 2^(120 - kLift - kLag), so that its product with a weight is finite.
 constexpr int kAim = 9;
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
         float mult;                     // factor of column g's scores, in units of log 2
         float q_sum[2][kWide ? G : 1];  // fp32: sums over the groups' channels of columns 2 j, 2 j + 1
         unsigned q_zero[2];             // two-byte types: the sums of column g as operand registers, against the zero points
-        bool spread = false;            // of a column, groups' largest channels are far apart
+        bool spread = false;            // products have units of their own: of a column, groups' largest channels are far apart, or it is very large
         int limit[2], own_limit;        // positions that the columns 2 j, 2 j + 1 see, and column g
         {
             float q[16];
@@ -459,6 +460,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                     const float own = s_most[warp * 8 + g];
                     if (own > 0.f && own < 0x1p-12f * most) unit = max(ka_exponent(own), all - 126);
                 }
+                const float times = pow2(max(unit - min(all, kMostQ), -126));
                 const float up = copysignf(pow2(14 - unit), p.scale);  // the scale's sign goes into q
                 float sum = 0.f;
 #pragma unroll
@@ -469,8 +471,8 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 sum += __shfl_xor_sync(kFullMask, sum, 1);
                 sum += __shfl_xor_sync(kFullMask, sum, 2);
                 if (j == 0) {
-                    s_qsum[g * G + warp] = sum * pow2(unit - all) * (kWide ? 1.f : pow2(-24));
-                    if (G > 1) s_qunit[g * G + warp] = pow2(unit - all);
+                    s_qsum[g * G + warp] = sum * pow2(-24) * times;
+                    s_qunit[g * G + warp] = times;
                 }
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {  // MMA m takes the codes 2 (m % 2), + 1, + 4, + 5 of word m / 2
@@ -486,12 +488,10 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             }
             __syncthreads();
             // not 0, so that a score of -infinity stays one
-            mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, (kWide ? 0 : 24) - 14 + ka_exponent(most)), 1e-37f);
-            if (G > 1) {  // in all warps alike: each looks at all columns
+            mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, 24 - 14 + min(ka_exponent(most), kMostQ)), 1e-37f);
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) spread |= s_qunit[g * G + gr] != 1.f;
-                spread = __any_sync(kFullMask, spread);
-            }
+            for (int gr = 0; gr < G; ++gr) spread |= s_qunit[g * G + gr] != 1.f;
+            spread = __any_sync(kFullMask, spread);  // in all warps alike: each looks at all columns
             // what belongs to a column, for the lanes that hold it in the products' layout: columns 2 j, 2 j + 1
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -615,14 +615,15 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                             float sum[4] = {0.f, 0.f, 0.f, 0.f};
                             ka_mma(sum, c0, c1, c2, c3, m ? b[1][gr].z : b[1][gr].x, m ? b[1][gr].w : b[1][gr].y);
                             ka_mma(sum, c0, c1, c2, c3, m ? b[0][gr].z : b[0][gr].x, m ? b[0][gr].w : b[0][gr].y);
-                            add_tile(acc[gr], sum);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[gr][i] = fmaf(sum[i], 0x1p-24f, acc[gr][i]);  // room for scales of any size
                         } else {
                             ka_mma(acc[gr], a0, a1, a2, a3, m ? b[0][gr].z : b[0][gr].x, m ? b[0][gr].w : b[0][gr].y);
                         }
                     }
                 }
             }
-            if (G > 1 && spread) {
+            if (spread) {
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr)
 #pragma unroll

@@ -221,3 +221,19 @@ def test_groups_of_a_query_may_be_of_any_size(cuda_device, dtype, d, hq, tokens)
         q = q.to(dtype)
         for scale in (0.2, -0.2):
             check_attention(s, q, mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu, scale=scale), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("power", [-120, -100, 100, 108, 120])
+def test_keys_may_be_of_any_size(cuda_device, dtype, d, power):
+    """Keys as large as queries are small, and the other way round: scores of an ordinary size."""
+    s = Server(cuda_device, dtype, d, 2, 32, [90, 17])
+    gen = torch.Generator().manual_seed(power + 200)
+    k, v = (torch.randn(107, 2, d, generator=gen).clamp(-3, 3) for _ in range(2))
+    q = torch.randn(2, 2, 4, d, generator=gen).clamp(-3, 3)
+    oracle.append(s.pool, s.table, s.lengths, (k * 2.0**power).to(dtype), v.to(dtype), s.lengths)
+    s.cache.pool.copy_(torch.from_numpy(s.pool))
+    q = (q * 2.0**-power).to(dtype)
+    check_attention(s, q, mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu))
