@@ -7,6 +7,7 @@
 // the reference's TORCH_CHECKs), allocates outputs, owns one workspace per device and passes raw
 // pointers and the current stream to libmk36; it contains no kernels and no arithmetic.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -713,6 +714,13 @@ std::tuple<torch::Tensor, torch::Tensor> kv4_read(torch::Tensor pool, torch::Ten
         k = part_of(both, sizes, 0), v = part_of(both, sizes, n);
     }
     TORCH_CHECK(k.sizes() == sizes, "out does not have the shape of the result");
+    if (k_out.has_value()) {  // a place that two tokens would be written to: either could come out
+        at::assert_no_internal_overlap(k);
+        at::assert_no_internal_overlap(v);
+        at::assert_no_overlap(k, v);
+        at::assert_no_overlap(k, pool);
+        at::assert_no_overlap(v, pool);
+    }
     mk36_kv4_tokens t = kv4_tokens(c, pool, k, v, cu_tokens);
     t.clear_rest = !k_out.has_value();
     if (k_out.has_value()) {

@@ -108,7 +108,7 @@ def kv4_read(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """The last ``tokens`` tokens of every row as dense keys and values ``[rows, tokens, kv_heads, head_dim]``; with
     ``cu_tokens`` (as in ``kv4_append``) ``[tokens, kv_heads, head_dim]``, ``tokens`` being the number for all rows.  ``out``: a
-    pair of tensors to write to; what lies behind the last row's tokens is left as it was there (0 without ``out``).  Positions before
+    pair of tensors to write to, without elements that share memory; what lies behind the last row's tokens is left as it was there (0 without ``out``).  Positions before
     a row's first token read as 0, positions without a page as NaN."""
     ext = _native("kv4_read", cache.pool, table.pages, table.lengths)
     if tokens < 0:
