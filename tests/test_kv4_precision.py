@@ -237,3 +237,49 @@ def test_keys_may_be_of_any_size(cuda_device, dtype, d, power):
     s.cache.pool.copy_(torch.from_numpy(s.pool))
     q = (q * 2.0**-power).to(dtype)
     check_attention(s, q, mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu))
+
+
+# What outputs may be off by before they are rounded, relative to their root mean square, on ordinary inputs (normal values, keys with a few channels
+# of mean 4, score sums of some 30 with rounding steps of 2^-24 by the dozen, divided by sqrt(d)): weights are off by some 5e-7 each, at random.
+# Zero points of bf16 meet weights of 16 bits: 2^-17 / sqrt(3) of zero points 2.5 times as large as the values.
+ORDINARY = {torch.float32: 2e-6, torch.float16: 3e-6, torch.bfloat16: 2.5e-5}
+
+
+def misrounded(out, want, dtype):
+    """Share of the outputs that are not `want` rounded to the type, and what it may be: an output is rounded elsewhere only if it lies within
+    its error of the middle between two neighbours.  Twice that share, for chance."""
+    nearest = want.to(dtype)
+    step = torch.finfo(dtype).eps * 2.0 ** torch.floor(torch.log2(want.abs().clamp_min(torch.finfo(dtype).smallest_normal)))
+    limit = 2 * (2 * ORDINARY[dtype] * want.square().mean().sqrt() / step).clamp_max(1).mean()
+    return (out != nearest).double().mean().item(), limit.item()
+
+
+def test_the_limits_for_ordinary_inputs_tell_halves_that_are_left_out():
+    """Outputs with the error of weights or queries of 11 bits (2^-12 / sqrt(3) at random, times zero points and codes 2.5 times as large as the values)
+    are beyond the limits, outputs with the error of the full kernel are not."""
+    gen = torch.Generator().manual_seed(1)
+    want = torch.randn(20000, generator=gen, dtype=torch.float64) * 0.05
+    noise = torch.randn(20000, generator=gen, dtype=torch.float64) * 0.05
+    for dtype in (torch.float16, torch.bfloat16):
+        share, limit = misrounded((want + noise * ORDINARY[dtype] / 2).to(dtype), want, dtype)
+        assert share <= limit
+        share, limit = misrounded((want + noise * 2.5 * 2.0**-12 / math.sqrt(3)).to(dtype), want, dtype)
+        assert share > limit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,hq,hkv,tokens", [(64, 8, 2, 1), (128, 16, 2, 1), (256, 16, 2, 1), (256, 24, 4, 3)])
+def test_ordinary_inputs_keep_all_digits(cuda_device, dtype, d, hq, hkv, tokens):
+    s = Server(cuda_device, dtype, d, hkv, 64, [700, 64, 33, 1500])
+    s.fill(seed=d)
+    q = torch.randn(4, tokens, hq, d, generator=torch.Generator().manual_seed(13)).to(dtype)
+    out = mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu).cpu()
+    want = oracle.attention(q, s.pool, s.table, s.lengths, dtype, d**-0.5)[0]
+    if dtype is torch.float32:
+        for r in range(4):
+            error = (out[r].double() - want[r]).square().mean().sqrt() / want[r].square().mean().sqrt()
+            assert error <= ORDINARY[dtype], f"row {r}: {error:.3g}"
+    else:
+        share, limit = misrounded(out, want, dtype)
+        assert share <= limit, f"{share:.4f} of the outputs, limit {limit:.4f}"
