@@ -487,8 +487,8 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 }
             }
             __syncthreads();
-            // not 0, so that a score of -infinity stays one
-            mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, 24 - 14 + min(ka_exponent(most), kMostQ)), 1e-37f);
+            // not 0, so that a score of -infinity stays one, but as near as can be, so that any other score times a scale of 0 is
+            mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, 24 - 14 + min(ka_exponent(most), kMostQ)), __uint_as_float(1u));
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) spread |= s_qunit[g * G + gr] != 1.f;
             spread = __any_sync(kFullMask, spread);  // in all warps alike: each looks at all columns

@@ -283,3 +283,16 @@ def test_ordinary_inputs_keep_all_digits(cuda_device, dtype, d, hq, hkv, tokens)
     else:
         share, limit = misrounded(out, want, dtype)
         assert share <= limit, f"{share:.4f} of the outputs, limit {limit:.4f}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [0.0, 2.0**-120])
+def test_a_scale_near_zero_takes_the_mean(cuda_device, dtype, scale):
+    s = Server(cuda_device, dtype, 64, 1, 16, [40, 5])
+    gen = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(45, 1, 64, generator=gen).clamp(-3, 3) for _ in range(2))
+    oracle.append(s.pool, s.table, s.lengths, (k * 2.0**120).to(dtype), v.to(dtype), s.lengths)
+    s.cache.pool.copy_(torch.from_numpy(s.pool))
+    q = (torch.randn(2, 3, 64, generator=gen).clamp(-3, 3) * 2.0**-14).to(dtype)  # scores of 2^112 before the scale
+    check_attention(s, q, mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu, scale=scale), scale)
