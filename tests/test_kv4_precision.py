@@ -296,3 +296,19 @@ def test_a_scale_near_zero_takes_the_mean(cuda_device, dtype, scale):
     s.cache.pool.copy_(torch.from_numpy(s.pool))
     q = (torch.randn(2, 3, 64, generator=gen).clamp(-3, 3) * 2.0**-14).to(dtype)  # scores of 2^112 before the scale
     check_attention(s, q, mk.kv4_attention_decode(q.to(cuda_device), s.cache, s.gpu, scale=scale), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("copies", [1, 300])
+def test_weights_of_any_size_count_where_the_largest_meets_zeros(cuda_device, dtype, d, copies):
+    """One token draws all but 2^-86 and has values of 0: the output is what the others leave.  (f16 holds weights at zero points down to 2^-31.)"""
+    row = Row(cuda_device, dtype, d, [100, 300, 16], copies=copies)
+    v = torch.randn(416, d, generator=torch.Generator().manual_seed(14))
+    codes = [0] * 416
+    for sink in (99, 100 + 140, 400):
+        codes[sink], v[sink] = 14, 0
+    row.fill(codes, v)
+    q = row.queries(4.25)
+    row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0), 4.25)
