@@ -191,8 +191,9 @@ __device__ __forceinline__ unsigned ka_keep(int t, int end) { return (t < end ? 
 // Weights are at most 2^(kLift + kLag).  f16 has them in two halves, for the zero points, and needs room below; the others hold them as fp32 and
 // as two bf16, and need room above: with weights of at most 1 no sum is larger than the values are.
 template <typename T>
-constexpr int kLift = std::is_same<T, __half>::value ? 7 : -4;
+constexpr int kLift = std::is_same<T, __half>::value ? 10 : -4;
 constexpr int kLag = 4;
+constexpr float kNoTop = -3e38f;  // below every score but -infinity, which then has a weight of 0
 constexpr int kMostQ = 100;  // queries larger than 2^100 have products in units of 2^100: the factor to log 2 units stays finite
 // Weights times scales of a group: the largest one is brought to 2^9 .. 2^10 and may grow to 2^15 before that is done again, by a power of two of
 // at most 2^(120 - kLift - kLag), so that its product with a weight is finite.
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
         float mult;                     // factor of column g's scores, in units of log 2
         float q_sum[2][kWide ? G : 1];  // fp32: sums over the groups' channels of columns 2 j, 2 j + 1
         unsigned q_zero[2];             // two-byte types: the sums of column g as operand registers, against the zero points
-        bool spread = false;            // products have units of their own: of a column, groups' largest channels are far apart, or it is very large
+        bool apart = false;             // groups' products have units of their own: of a column, their largest channels are far apart, or it is very large
         int limit[2], own_limit;        // positions that the columns 2 j, 2 j + 1 see, and column g
         {
             float q[16];
@@ -490,8 +491,8 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             // not 0, so that a score of -infinity stays one, but as near as can be, so that any other score times a scale of 0 is
             mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, 24 - 14 + min(ka_exponent(most), kMostQ)), __uint_as_float(1u));
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) spread |= s_qunit[g * G + gr] != 1.f;
-            spread = __any_sync(kFullMask, spread);  // in all warps alike: each looks at all columns
+            for (int gr = 0; gr < G; ++gr) apart |= s_qunit[g * G + gr] != 1.f;
+            apart = __any_sync(kFullMask, apart);  // in all warps alike: each looks at all columns
             // what belongs to a column, for the lanes that hold it in the products' layout: columns 2 j, 2 j + 1
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -514,7 +515,6 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                     const float2 f = KaPair<T>::unpack(part[i]);
                     x[0] -= f.x, x[1] -= f.y;
                 }
-                if (spread) part[0] = part[1] = part[2] = part[3] = 0u;  // in fp32 with the products, below
                 const bool second = j >> 1;
                 q_zero[0] = second ? part[1] : part[0];
                 q_zero[1] = std::is_same<T, __half>::value ? 0u : (second ? part[3] : part[2]);
@@ -526,9 +526,8 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
 
         // zero_sum: the zero points' part, of column g for every group (fp32), or as an MMA leaves it: row g % 4 (the group), columns 2 j, 2 j + 1
         constexpr int Z = kWide ? G : 4;
-        // top: what weights are relative to, a whole number of log 2 units no less than the maximum less kLag; shift: kLift - top.  up: the power of
-        // two of weights times scales, of column g
-        float o[G][4][4], zero_sum[Z], up[G], top = -INFINITY, shift = 0.f, weight_sum = 0.f;
+        // top: the score that weights are relative to, no further than kLag below the maximum; up: the power of two of weights times scales, of column g
+        float o[G][4][4], zero_sum[Z], up[G], top = kNoTop, weight_sum = 0.f;
 #pragma unroll
         for (int i = 0; i < Z; ++i) zero_sum[i] = 0.f;
 #pragma unroll
@@ -539,16 +538,15 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[gr][m][i] = 0.f;
         }
-        // Brings the sums of the codes down by 2^-by[group], of column g each.
-        auto bring_down = [&](const int (&by)[G]) {
+        // Brings the sums of the codes down by a factor for each group, of column g.
+        auto bring_down = [&](const float (&by)[G]) {
             bool some = false;
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) some |= by[gr] != 0;
+            for (int gr = 0; gr < G; ++gr) some |= by[gr] != 1.f;
             if (!__any_sync(kFullMask, some)) return;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-                const float f = pow2(-min(by[gr], 126));
-                const float c0 = __shfl_sync(kFullMask, f, 8 * j), c1 = __shfl_sync(kFullMask, f, 8 * j + 4);
+                const float c0 = __shfl_sync(kFullMask, by[gr], 8 * j), c1 = __shfl_sync(kFullMask, by[gr], 8 * j + 4);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     o[gr][m][0] *= c0, o[gr][m][1] *= c1;
@@ -623,23 +621,27 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                     }
                 }
             }
-            if (spread) {
+            if (apart) {  // zero points in fp32 too
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float* unit = &s_qunit[(2 * j + (i & 1)) * G];
+                    const float* sum = &s_qsum[(2 * j + (i & 1)) * G];
+                    s[i] = 0.f;
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        s[i] = fmaf(kWide ? fmaf(8.f, ks[i >> 1][gr], kz[i >> 1][gr]) : kz[i >> 1][gr], sum[gr], s[i]);
+                        s[i] = fmaf(ks[i >> 1][gr], acc[gr][i] * unit[gr], s[i]);
+                    }
+                }
+            } else {
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int at_q = (2 * j + (i & 1)) * G + gr;
-                        acc[gr][i] *= s_qunit[at_q];
-                        if constexpr (!kWide) s[i] = fmaf(kz[i >> 1][gr], s_qsum[at_q], s[i]);
+                        if constexpr (kWide) s[i] = fmaf(fmaf(8.f, ks[i >> 1][gr], kz[i >> 1][gr]), q_sum[i & 1][gr], s[i]);
+                        s[i] = fmaf(ks[i >> 1][gr], acc[gr][i], s[i]);
                     }
             }
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (kWide) s[i] = fmaf(fmaf(8.f, ks[i >> 1][gr], kz[i >> 1][gr]), q_sum[i & 1][gr], s[i]);
-                    s[i] = fmaf(ks[i >> 1][gr], acc[gr][i], s[i]);
-                }
             const bool edge = first + kKv4Tile > sees_all;
             if (edge) {
 #pragma unroll
@@ -651,14 +653,14 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             transpose8(s[2], s[3]);
 
             // ---- maximum.  `top` follows it only when it is 2^kLag times larger: then, and not with every tile, what has been summed is brought
-            // to the new one.
+            // to the new one.  Differences of scores come first: they are exact where they matter, for scores of any size.
             float most = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-            if (__any_sync(kFullMask, fmaf(most, mult, -(float)kLag) > top)) {
+            if (__any_sync(kFullMask, (most - top) * mult > (float)kLag)) {
                 most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
-                const float next = fmaxf(top, ceilf(most * mult)), next_shift = next == -INFINITY ? 0.f : kLift<T> - next;
-                const float drop = top == -INFINITY ? 0.f : shift - next_shift, corr = exp2f(-drop);  // nothing has been summed without a maximum
-                top = next, shift = next_shift;
+                const float next = fmaxf(top, most), drop = (next - top) * mult;
+                const float corr = exp2f(-drop);
+                top = next;
                 weight_sum *= corr;
                 if constexpr (kWide) {
 #pragma unroll
@@ -666,19 +668,23 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 } else {
                     zero_sum[0] *= __shfl_sync(kFullMask, corr, 8 * j), zero_sum[1] *= __shfl_sync(kFullMask, corr, 8 * j + 4);
                 }
-                // weights get smaller, `up` grows by as much, and the sums stay as they are; at its end they get smaller
+                // weights get smaller, and `up` grows by as much as far as it goes and in whole powers of two; the rest is the sums'
                 const int by = (int)fminf(drop, 1000.f);
-                int rest[G];
+                const float part = exp2f((float)by - drop);
+                float rest[G];
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
                     const int e = exponent_of(up[gr]), n = min(e + by, kMostUp<T>);
                     up[gr] = pow2(n);
-                    rest[gr] = e + by - n;
+                    rest[gr] = pow2(max(n - e - by, -126)) * part;
                 }
-                bring_down(rest);
+                if (!fresh) bring_down(rest);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = kWide ? exp2f(fmaf(s[i], mult, shift)) : exp2_approx(fmaf(s[i], mult, shift));
+            for (int i = 0; i < 4; i += 2) {
+                const f32x2 x = fma_pair(add_pair(pair_of(s[i], s[i + 1]), pair_of(-top, -top)), pair_of(mult, mult), pair_of((float)kLift<T>, (float)kLift<T>));
+                s[i] = kWide ? exp2f(first_of(x)) : exp2_approx(first_of(x)), s[i + 1] = kWide ? exp2f(second_of(x)) : exp2_approx(second_of(x));
+            }
             weight_sum += (s[0] + s[1]) + (s[2] + s[3]);
 
             // ---- scales of the values of the lane's four tokens; what the column does not see may be anything, a NaN too
@@ -724,7 +730,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 }
                 const bool fits = __hbleu2(largest, __float2half2_rn(32768.f));
                 if (turn == 1 || __all_sync(kFullMask, fits)) break;
-                int by[G];
+                float by[G];
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
                     float m = 0.f;  // 2^-20 of the largest, which is finite
@@ -735,7 +741,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                     const int e = exponent_of(up[gr]), size = exponent_of(m) + 20;
                     const int n = m == 0.f ? e : max(min(e, kAim - size), -126);
                     up[gr] = pow2(n);
-                    by[gr] = e - n;
+                    by[gr] = pow2(max(n - e, -126));
                 }
                 if (!fresh) bring_down(by);
             }
@@ -837,7 +843,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
         }
         if (j == 0) {
             const int c = warp * 8 + g;
-            s_max[c] = top == -INFINITY ? top : -shift;
+            s_max[c] = fminf(fmaxf(top * mult, kNoTop), -kNoTop);
             s_sum[c] = weight_sum;
         }
         __syncthreads();

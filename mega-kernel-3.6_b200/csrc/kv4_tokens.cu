@@ -139,17 +139,6 @@ __device__ __forceinline__ unsigned codes_exact(const float (&x)[8], float zero,
     return four_exact(make_float4(x[0], x[1], x[2], x[3]), zero, scale) | four_exact(make_float4(x[4], x[5], x[6], x[7]), zero, scale) << 16;
 }
 
-__device__ __forceinline__ f32x2 add_pair(f32x2 a, f32x2 b) {
-    f32x2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ f32x2 fma_pair(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
 constexpr float kRoundUp = 12582912.0f;  // 1.5 * 2^23: added, it rounds to a whole number, halves to even, and leaves that in the low bits
 
 // Whole numbers below 16, as floats, to a word of eight half bytes: sums of four are exact.

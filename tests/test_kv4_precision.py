@@ -312,3 +312,21 @@ def test_weights_of_any_size_count_where_the_largest_meets_zeros(cuda_device, dt
     row.fill(codes, v)
     q = row.queries(4.25)
     row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=1.0), 4.25)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,copies", [(64, 1), (128, 300), (256, 300)])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+def test_scores_of_any_size(cuda_device, dtype, d, copies, order):
+    """Scores so far apart that the largest draws everything, up to 2^100: tokens of the largest score share the output."""
+    n = 240
+    codes = {"rising": [i // 16 for i in range(n)], "falling": [14 - i // 16 for i in range(n)],
+             "mixed": torch.randint(0, 15, (n,), generator=torch.Generator().manual_seed(4)).tolist()}[order]
+    row = Row(cuda_device, dtype, d, [n], copies=copies)
+    row.fill(codes, torch.randn(n, d, generator=torch.Generator().manual_seed(15)))
+    for power in (4, 10, 14, 19, 24, 28, 33, 40, 60, 100):
+        for sign in (1, -1):
+            step, scale = (2.0**10, 2.0 ** (power - 10)) if power > 10 else (2.0**power, 1.0)
+            q = row.queries(sign * step, tokens=2)
+            row.check(q, mk.kv4_attention_decode(q.to(cuda_device), row.cache, row.gpu, scale=scale), sign * step * scale)
