@@ -659,26 +659,28 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(kFullMask, most, 2));
                 const float next = fmaxf(top, most), drop = (next - top) * mult;
-                const float corr = exp2f(-drop);
                 top = next;
-                weight_sum *= corr;
-                if constexpr (kWide) {
+                if (!fresh) {
+                    const float corr = exp2f(-drop);
+                    weight_sum *= corr;
+                    if constexpr (kWide) {
 #pragma unroll
-                    for (int gr = 0; gr < G; ++gr) zero_sum[gr] *= corr;
-                } else {
-                    zero_sum[0] *= __shfl_sync(kFullMask, corr, 8 * j), zero_sum[1] *= __shfl_sync(kFullMask, corr, 8 * j + 4);
-                }
-                // weights get smaller, and `up` grows by as much as far as it goes and in whole powers of two; the rest is the sums'
-                const int by = (int)fminf(drop, 1000.f);
-                const float part = exp2f((float)by - drop);
-                float rest[G];
+                        for (int gr = 0; gr < G; ++gr) zero_sum[gr] *= corr;
+                    } else {
+                        zero_sum[0] *= __shfl_sync(kFullMask, corr, 8 * j), zero_sum[1] *= __shfl_sync(kFullMask, corr, 8 * j + 4);
+                    }
+                    // weights get smaller, and `up` grows by as much as far as it goes and in whole powers of two; the rest is the sums'
+                    const int by = (int)fminf(drop, 1000.f);
+                    const float part = exp2f((float)by - drop);
+                    float rest[G];
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) {
-                    const int e = exponent_of(up[gr]), n = min(e + by, kMostUp<T>);
-                    up[gr] = pow2(n);
-                    rest[gr] = pow2(max(n - e - by, -126)) * part;
+                    for (int gr = 0; gr < G; ++gr) {
+                        const int e = exponent_of(up[gr]), n = min(e + by, kMostUp<T>);
+                        up[gr] = pow2(n);
+                        rest[gr] = pow2(max(n - e - by, -126)) * part;
+                    }
+                    bring_down(rest);
                 }
-                if (!fresh) bring_down(rest);
             }
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
