@@ -466,8 +466,8 @@ typedef struct mk36_kv4_tokens {
 } mk36_kv4_tokens;
 
 /* Quantises and writes them.  Of a group: zero = the least value, scale = (greatest - least) / 15 rounded to dtype, code =
- * (value - zero) / scale rounded to the nearest (halves to even), at most 15, all of it exact before each rounding; codes are 0 where
- * the scale is 0.  A group with an infinity or a NaN stands for NaN.  Tokens without a place (position below zero, no page or one
+ * (value - zero) / scale rounded to the nearest (halves to even), at most 15, before each rounding exact for the two-byte types and in
+ * 64 bits for fp32; codes are 0 where the scale is 0.  A group with an infinity or a NaN stands for NaN.  Tokens without a place (position below zero, no page or one
  * outside the pool, behind the last row) are not written.  No two rows may hold the page that a token is written to. */
 MK36_API int mk36_kv4_append(const mk36_kv4_cache* cache, const mk36_kv4_tokens* tokens, void* stream);
 /* Reads them back, rounded once; tokens of a position below zero come back as zeros, those without a page in the pool as NaN, and
@@ -476,7 +476,8 @@ MK36_API int mk36_kv4_read(const mk36_kv4_cache* cache, const mk36_kv4_tokens* t
 
 /* Attention of the last `tokens` tokens of every row over the row: q, out [rows, tokens, query_heads, head_dim] (out dense, q
  * with strides in elements and contiguous channels), token i of a row sees the positions 0 .. lengths[r] - tokens + i.  A
- * query that sees nothing gives zeros; one that reaches a page outside the pool gives NaN.  The workspace is scratch for this call
+ * query that sees nothing gives zeros; one that reaches a page outside the pool gives NaN.  Keys, values and queries may be of any finite
+ * size, also by token and by group of 64 channels; of f16, weights below 2^-35 of the largest do not count at the zero points.  The workspace is scratch for this call
  * alone (it need not be initialised): two calls that may overlap, or two captured graphs, have one each. */
 typedef struct mk36_kv4_attention_args {
     const void* q;
@@ -499,10 +500,12 @@ MK36_API int mk36_kv4_attention_decode(const mk36_kv4_cache* cache, const mk36_k
  *   resize  row r goes from lengths[r] to new_lengths[r] tokens.  Pages behind its new end lose a reference and its entries become
  *           -1; then a row that grows, and whose last page is filled in part and shared, gets a copy of it (the tiles that hold tokens), and
  *           new pages are taken, lowest free number first, in the order of rows and, in a row, the copy first.  Status n > 0: n pages
- *           are missing; -1: a length below 0 or beyond row_pages * page_size, or an entry outside the pool where a page is held.
+ *           are missing; -1: a length below 0 or beyond row_pages * page_size, or an entry outside the pool where a page would be freed
+ *           or copied.  Where all rows that hold a page grow, each gets a copy and the page itself is free after the call.
  *   compact pages in use behind the first n, n the number of pages in use, move to the free ones among the first n, both
  *           ascending; *status = n.
- * pool, kv_heads, page_size and tile_bytes are those of the cache (resize, compact). */
+ * pool, kv_heads, page_size and tile_bytes are those of the cache (resize, compact).  Layers that share a table have a pool each: every
+ * layer's call takes the same *_in and gives the same *_out, and only the last one's *_out may be the same arrays as its *_in. */
 typedef struct mk36_kv_pages_args {
     const int32_t* page_table_in;
     const int32_t* lengths_in;

@@ -13,6 +13,10 @@ A serving step with it::
 
 All tables live on the GPU and no call waits for the host, so steps can be captured into CUDA graphs; a captured call
 follows what the tables hold at replay.
+
+Layers that share a table have a pool each.  ``kv_pages_resize`` and ``kv_pages_compact`` copy and move the pages of the pool that they
+are given, by the table as it was before: call them for every layer with that same table, each call gives the same new one, and only
+the last may be in place.  A layer that gets the new table instead has no pages copied, and nothing says so.
 """
 
 from __future__ import annotations
@@ -91,7 +95,7 @@ def kv4_append(cache: Kv4Cache, table: PageTable, k: torch.Tensor, v: torch.Tens
     kv_heads, head_dim]``, row r having tokens ``cu_tokens[r]`` to ``cu_tokens[r + 1] - 1``; tokens behind the last row's are
     padding.  Only the channels need to be contiguous.  Of a group of 64 channels the zero point is the least value, the scale
     ``(greatest - least) / 15`` rounded to the cache's type, and a code ``(value - zero) / scale`` rounded to the nearest (halves to
-    even), at most 15.  A group with an infinity or a NaN stands for NaN.  A token without a page (-1) is not written.  Pages that
+    even), at most 15; float32 takes the difference in 64 bits.  A group with an infinity or a NaN stands for NaN.  A token without a page (-1) is not written.  Pages that
     are written must not be shared: ``kv_pages_resize`` sees to that."""
     ext = _native("kv4_append", cache.pool, table.pages, table.lengths, k, v)
     _check_dtype(cache, k, v)
@@ -123,7 +127,8 @@ def kv4_attention_decode(q: torch.Tensor, cache: Kv4Cache, table: PageTable, *, 
     """Grouped-query attention of each row's last token, q ``[rows, query_heads, head_dim]``, or of its last tokens, q ``[rows,
     tokens, query_heads, head_dim]`` (a draft being checked, a prompt's end), over the row; token i of ``tokens`` sees the positions up
     to its own, ``lengths - tokens + i``.  ``scale`` is 1 / sqrt(head_dim) by default.  A query that sees nothing (an empty row)
-    gives zeros, one that meets a page outside the pool NaN."""
+    gives zeros, one that meets a page outside the pool NaN.  Keys, values and queries may be of any finite size, also by token and by group of
+    64 channels; of float16, weights below 2^-35 of the largest do not count at the zero points."""
     ext = _native("kv4_attention_decode", q, cache.pool, table.pages, table.lengths)
     _check_dtype(cache, q)
     if scale is None:
@@ -148,8 +153,9 @@ def kv_pages_resize(cache: Kv4Cache, table: PageTable, new_lengths: torch.Tensor
     """Takes and frees pages so that every row has room for ``new_lengths`` (int32) tokens: 0 ends a row, fewer tokens take some
     back, more make room for an append.  A row that grows gets a copy of its last page where other rows hold that page too and it is
     filled in part.  Free pages are taken lowest number first, row after row.  Returns the new table and an int32 status ``[1]``
-    on the device: 0; n > 0 where n pages are missing; -1 for a length outside the table or a held entry outside the pool.  Where
-    it is not 0 nothing has changed."""
+    on the device: 0; n > 0 where n pages are missing; -1 for a length outside the table, or for an entry outside the pool where a page
+    would be freed or copied.  Where it is not 0 nothing has changed.  Where all the rows that hold a page grow, each gets a copy, and the page
+    itself is free after the call."""
     ext = _native("kv_pages_resize", cache.pool, table.pages, table.lengths, table.refcounts, new_lengths)
     return _result(table, inplace, ext.kv_pages_resize(cache.pool, table.pages, table.lengths, table.refcounts, new_lengths, bool(inplace)))
 
