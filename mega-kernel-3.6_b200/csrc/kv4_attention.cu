@@ -15,6 +15,8 @@
 //     that this query does not see.  They are held in two halves (hi + lo, 22 bits, and down to 2^-34 of the largest): a rounded weight's error would be
 //     multiplied by a code of 0 .. 15 where the value itself, with its zero point, may be near zero.  (One half: 6 us of 78 less at 48 long
 //     rows, and an error of 2^-11 of the codes' size.)
+//   * Weights at the zero points are of the operands' type: two halves of f16 (22 bits, and down to 2^-35 of the largest weight) or of bf16 (16 bits; the
+//     output has 8, and what lies next to the middle between two neighbours may go to the other one); fp32 multiplies them as they are.
 //   * fp32 splits its queries the same way, takes codes less 8, and adds up short chains of products in fp32 (its error against 64 bits
 //     is 2e-7 to 5e-7 of the output, that of sums in fp32 throughout 2e-7 to 9e-7).
 //
@@ -26,9 +28,9 @@
 // leaves a partial result, and a second launch, set up while the first still runs, joins those.
 //
 // What bounds it.  Short rows: latency, 9.6 us for one row of 700 tokens.  Many long rows: not memory (tiles that all lie in L2 take 97 % of
-// the time) but the SMs: 632 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
+// the time) but the SMs: 644 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
 // of 8 cycles; issue slots, that pipe, the tensor cores and shared memory are each 40 to 60 % busy, with three warps a scheduler.  48 rows
-// of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78 us, 3.5 TB/s; 24 / 4 heads, three tokens, 12 rows: 43.1 us.
+// of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78.5 us, 3.5 TB/s, whatever the size of the values; 24 / 4 heads, three tokens, 12 rows: 43.8 us.
 #include <math.h>
 
 #include <type_traits>
@@ -950,7 +952,7 @@ __device__ __forceinline__ void ka_join_batch(const float* values, const float* 
 //
 // Few passes: a CTA of 32 warps takes 64 channels of one query head and token.  A warp takes every 32nd partial result, kBatch of them in
 // flight together, with a running maximum of its own: a round trip for a batch is 2 to 3 us (one row of 32768 tokens, 16 / 2 heads of 256,
-// 205 partial results for each: 16.7 us for the call, 19.1 with the other form; one of 700 tokens 8.8 and 9.0).
+// 205 partial results for each: 16.8 us for the call with the cache in L2, 19.6 with the other form; one of 700 tokens 8.4 and 8.5).
 constexpr int kKaWideWarps = 32;
 
 template <typename T, int D>
@@ -1008,8 +1010,8 @@ __global__ void __launch_bounds__(kKaWideWarps * 32) kv4_attention_join_wide_ker
 }
 
 // Any others: a CTA for each cut of the line, and those of one pass share its eight columns and their groups of 64 channels.  Passes that
-// are whole cost nothing (a CTA for each query head took 35 us where this takes 26: 256 rows of 500 tokens, 16 / 2 heads of 128; 57 and 24
-// for 1024 rows of 7).  With eight partial results in flight for a warp, not three, 74 registers leave room for three CTAs an SM: 30 us.
+// are whole cost nothing (a CTA of a few warps for each query head took 35 us where this takes 25: 256 rows of 500 tokens, 16 / 2 heads of
+// 128; 57 and 24 for 1024 rows of 7; but 46.8 and 48.2 for eight rows of 32768, and 42.9 and 43.3 for 12 rows of 27B heads with three tokens).  With eight partial results in flight for a warp, not three, 74 registers leave room for three CTAs an SM: 30 us.
 constexpr int kKaJoinWarps = 8;
 
 template <typename T, int D>
@@ -1105,8 +1107,8 @@ static int ka_grid(Kv4AttnParams* p, const mk36_kv4_cache* c) {
     const long long most = (long long)line;
     const long long ctas = (most + kKaMinTiles - 1) / kKaMinTiles, resident = (long long)info->sm_count * ka_ctas_per_sm(c->dtype == MK36_F32, c->head_dim);
     p->ctas = (int)(ctas < resident ? ctas : resident);
-    // The wide form of the join: more than 64 pieces a pass when the table is full (4 rows, 16 / 2 heads of 128, 74 pieces: 15.0 us, 17.0 with
-    // the other; 2 rows, 24 / 4 heads of 256, 55 pieces: 30.4 and 30.2), or an SM for each CTA of both launches.  Either way there
+    // The wide form of the join: more than 64 pieces a pass when the table is full (4 rows, 16 / 2 heads of 128, 74 pieces: 14.5 us, 15.8 with
+    // the other; 2 rows, 24 / 4 heads of 256, 55 pieces: 30.4 and 29.6; 8 rows, 16 / 2 heads of 256, 28 pieces: 55.5 and 48.2), or an SM for each CTA of both launches.  Either way there
     // are at most two such CTAs for each SM.
     const long long outputs = (long long)p->cache.rows * p->tokens * p->query_heads;
     p->join_wide = p->ctas > 64ll * p->cache.rows * p->streams || p->ctas + outputs * (c->head_dim / 64) <= info->sm_count;

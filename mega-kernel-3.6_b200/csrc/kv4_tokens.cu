@@ -5,10 +5,12 @@
 // append has 16 channels for a thread (32 bytes of a 2-byte type on one side, two 32-bit words of codes on the other), four threads a
 // group, whose minimum and maximum travel as one pair through two shuffles; a read has eight.
 //
-// Codes and scales follow from exact arithmetic, whatever the order of operations in fp32 would give: see codes_of and scale_of.
+// Codes and scales follow from exact arithmetic (fp32: from 64 bits), whatever the order of operations in fp32 would give: see codes_of and
+// scale_of.
 //
-// What bounds them: reading back, memory and instructions alike (32768 tokens of 2 heads of 256 in bf16: 83 MB in 16.3 us, 5.1 TB/s);
-// appending, instructions (28.7 us, 2.9 TB/s; 26.2 us in f16, where fewer values lie half way between codes).
+// What bounds them: reading back, memory and instructions alike (32768 tokens of 2 heads of 256 in bf16: 86 MB in 16.3 us, 5.3 TB/s; in fp32
+// 155 MB in 36 us, 4.3 TB/s); appending, instructions (28.7 us, 3.0 TB/s; 26.2 us in f16, where fewer values lie half way between codes; fp32 41.9
+// us, 3.7 TB/s).
 #include <type_traits>
 
 #include "mk36_kv4.cuh"
