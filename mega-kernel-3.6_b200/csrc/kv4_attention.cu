@@ -195,7 +195,7 @@ __device__ __forceinline__ unsigned ka_keep(int t, int end) { return (t < end ? 
 template <typename T>
 constexpr int kLift = std::is_same<T, __half>::value ? 10 : -4;
 constexpr int kLag = 4;
-constexpr float kNoTop = -3e38f;  // below every score but -infinity, which then has a weight of 0
+constexpr float kNoTop = -3e38f;  // below every score but -infinity, which then has a weight of 0; sums without a maximum are 0 or NaN, and finite factors keep them
 constexpr int kMostQ = 100;  // queries larger than 2^100 have products in units of 2^100: the factor to log 2 units stays finite
 // Weights times scales of a group: the largest one is brought to 2^9 .. 2^10 and may grow to 2^15 before that is done again, by a power of two of
 // at most 2^(120 - kLift - kLag), so that its product with a weight is finite.
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
 #pragma unroll
             for (int w = 0; w < kKaWarps; ++w) m = fmaxf(m, s_max[w * 8 + 2 * j + c]);
             const float own = s_max[warp * 8 + 2 * j + c];
-            const float weight = own == -INFINITY ? 0.f : exp2f(own - m);
+            const float weight = exp2f(own - m);
             // channel 8 g + i of a group at 8 i + g
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
 #pragma unroll
                 for (int w = 0; w < kKaWarps; ++w) {
                     const int x = w * 8 + mine;
-                    sum += s_max[x] == -INFINITY ? s_sum[x] : exp2f(s_max[x] - most) * s_sum[x];  // without a maximum the sum is 0 or NaN
+                    sum += exp2f(s_max[x] - most) * s_sum[x];
                 }
                 const int token = fdiv(column, p.fd_group), head = kv_head * p.group + column - token * p.group;
                 T* out = static_cast<T*>(p.out) + (((long long)row * p.tokens + token) * p.query_heads + head) * D;
@@ -924,7 +924,7 @@ __device__ __forceinline__ void ka_join(const float2 (&stats)[N], const float2 (
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float own = exp2f(stats[i].x - base);
-        sum += stats[i].x == -INFINITY ? stats[i].y : own * stats[i].y;  // without a maximum the sum is 0 or NaN
+        sum = fmaf(own, stats[i].y, sum);
         acc.x = fmaf(own, value[i].x, acc.x), acc.y = fmaf(own, value[i].y, acc.y);
     }
 }
