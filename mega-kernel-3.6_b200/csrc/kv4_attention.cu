@@ -27,10 +27,10 @@
 // tiles of all rows and heads form one line that is cut into as many equal pieces as there are CTAs; a piece that ends inside a row
 // leaves a partial result, and a second launch, set up while the first still runs, joins those.
 //
-// What bounds it.  Short rows: latency, 9.6 us for one row of 700 tokens.  Many long rows: not memory (tiles that all lie in L2 take 97 % of
-// the time) but the SMs: 644 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
+// What bounds it.  Short rows: latency, 8.9 us for one row of 700 tokens.  Many long rows: not memory (tiles that all lie in L2 take 97 % of
+// the time) but the SMs: 642 instructions a tile, half of them masks, shifts and permutations that issue every other cycle, 51 MMAs
 // of 8 cycles; issue slots, that pipe, the tensor cores and shared memory are each 40 to 60 % busy, with three warps a scheduler.  48 rows
-// of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78.5 us, 3.5 TB/s, whatever the size of the values; 24 / 4 heads, three tokens, 12 rows: 43.8 us.
+// of 2000 to 40000 tokens, 16 / 2 heads of 256: 273 MB in 78.1 us, 3.5 TB/s, whatever the size of the values; 24 / 4 heads, three tokens, 12 rows: 43.2 us.
 #include <math.h>
 
 #include <type_traits>
@@ -43,7 +43,7 @@ namespace mk36 {
 
 constexpr int kKaWarps = 4;
 constexpr int kKaThreads = kKaWarps * 32;
-constexpr int kKaMinTiles = kKaWarps;  // fewest tiles of a piece: one a warp (one row of 700 tokens: 9.6 us; two a warp 12.6, four 14.8)
+constexpr int kKaMinTiles = kKaWarps;  // fewest tiles of a piece: one a warp (one row of 700 tokens, when it was chosen: 9.6 us; two a warp 12.6, four 14.8)
 
 struct Kv4AttnParams {
     Kv4View cache;
@@ -952,7 +952,7 @@ __device__ __forceinline__ void ka_join_batch(const float* values, const float* 
 //
 // Few passes: a CTA of 32 warps takes 64 channels of one query head and token.  A warp takes every 32nd partial result, kBatch of them in
 // flight together, with a running maximum of its own: a round trip for a batch is 2 to 3 us (one row of 32768 tokens, 16 / 2 heads of 256,
-// 205 partial results for each: 16.8 us for the call with the cache in L2, 19.6 with the other form; one of 700 tokens 8.4 and 8.5).
+// 205 partial results for each: 15.9 us for the call with the cache in L2, 19.8 with the other form; one of 700 tokens 8.0 and 8.5).
 constexpr int kKaWideWarps = 32;
 
 template <typename T, int D>
@@ -1010,8 +1010,8 @@ __global__ void __launch_bounds__(kKaWideWarps * 32) kv4_attention_join_wide_ker
 }
 
 // Any others: a CTA for each cut of the line, and those of one pass share its eight columns and their groups of 64 channels.  Passes that
-// are whole cost nothing (a CTA of a few warps for each query head took 35 us where this takes 25: 256 rows of 500 tokens, 16 / 2 heads of
-// 128; 57 and 24 for 1024 rows of 7; but 46.8 and 48.2 for eight rows of 32768, and 42.9 and 43.3 for 12 rows of 27B heads with three tokens).  With eight partial results in flight for a warp, not three, 74 registers leave room for three CTAs an SM: 30 us.
+// are whole cost nothing (a CTA of a few warps for each query head took 35 us where this takes 24: 256 rows of 500 tokens, 16 / 2 heads of
+// 128; 57 and 23 for 1024 rows of 7; but 46.8 and 47.6 for eight rows of 32768, and 42.9 and 43.2 for 12 rows of 27B heads with three tokens).  With eight partial results in flight for a warp, not three, 74 registers leave room for three CTAs an SM: 30 us.
 constexpr int kKaJoinWarps = 8;
 
 template <typename T, int D>
@@ -1107,8 +1107,8 @@ static int ka_grid(Kv4AttnParams* p, const mk36_kv4_cache* c) {
     const long long most = (long long)line;
     const long long ctas = (most + kKaMinTiles - 1) / kKaMinTiles, resident = (long long)info->sm_count * ka_ctas_per_sm(c->dtype == MK36_F32, c->head_dim);
     p->ctas = (int)(ctas < resident ? ctas : resident);
-    // The wide form of the join: more than 64 pieces a pass when the table is full (4 rows, 16 / 2 heads of 128, 74 pieces: 14.5 us, 15.8 with
-    // the other; 2 rows, 24 / 4 heads of 256, 55 pieces: 30.4 and 29.6; 8 rows, 16 / 2 heads of 256, 28 pieces: 55.5 and 48.2), or an SM for each CTA of both launches.  Either way there
+    // The wide form of the join: more than 64 pieces a pass when the table is full (4 rows, 16 / 2 heads of 128, 74 pieces: 13.7 us, 15.2 with
+    // the other; 2 rows, 24 / 4 heads of 256, 55 pieces: 29.5 and 28.9; 8 rows, 16 / 2 heads of 256, 28 pieces: 54.7 and 47.6), or an SM for each CTA of both launches.  Either way there
     // are at most two such CTAs for each SM.
     const long long outputs = (long long)p->cache.rows * p->tokens * p->query_heads;
     p->join_wide = p->ctas > 64ll * p->cache.rows * p->streams || p->ctas + outputs * (c->head_dim / 64) <= info->sm_count;
