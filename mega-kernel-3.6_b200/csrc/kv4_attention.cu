@@ -456,14 +456,18 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             most = 0.f;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) most = fmaxf(most, s_most[gr * 8 + g]);
-            if (warp < G) {
-                const int all = ka_exponent(most);
-                int unit = all;
-                if (G > 1) {
-                    const float own = s_most[warp * 8 + g];
-                    if (own > 0.f && own < 0x1p-12f * most) unit = max(ka_exponent(own), all - 126);
+            // The unit of the column's products: such that the groups' own units are within 2^-126 .. 2^127 of it.
+            const int all = ka_exponent(most);
+            int unit = all, column_unit = min(all, kMostQ);
+#pragma unroll
+            for (int gr = 0; G > 1 && gr < G; ++gr) {
+                const float own = s_most[gr * 8 + g];
+                if (own > 0.f && own < 0x1p-12f * most) {
+                    column_unit = min(column_unit, ka_exponent(own) + 126);
+                    if (gr == warp) unit = ka_exponent(own);
                 }
-                const float times = pow2(max(unit - min(all, kMostQ), -126));
+            }
+            if (warp < G) {
                 const float up = copysignf(pow2(14 - unit), p.scale);  // the scale's sign goes into q
                 float sum = 0.f;
 #pragma unroll
@@ -474,8 +478,8 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                 sum += __shfl_xor_sync(kFullMask, sum, 1);
                 sum += __shfl_xor_sync(kFullMask, sum, 2);
                 if (j == 0) {
-                    s_qsum[g * G + warp] = sum * pow2(-24) * times;
-                    s_qunit[g * G + warp] = times;
+                    s_qsum[g * G + warp] = sum * pow2(-24);
+                    s_qunit[g * G + warp] = pow2(unit - column_unit);
                 }
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {  // MMA m takes the codes 2 (m % 2), + 1, + 4, + 5 of word m / 2
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
             }
             __syncthreads();
             // not 0, so that a score of -infinity stays one, but as near as can be, so that any other score times a scale of 0 is
-            mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, 24 - 14 + min(ka_exponent(most), kMostQ)), __uint_as_float(1u));
+            mult = fmaxf(ldexpf(fabsf(p.scale) * 1.4426950408889634f, 24 - 14 + column_unit), __uint_as_float(1u));
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) apart |= s_qunit[g * G + gr] != 1.f;
             apart = __any_sync(kFullMask, apart);  // in all warps alike: each looks at all columns
@@ -631,8 +635,8 @@ __global__ void __launch_bounds__(kKaThreads, KaConfig<T, D>::kCtas) kv4_attenti
                     s[i] = 0.f;
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
-                        s[i] = fmaf(kWide ? fmaf(8.f, ks[i >> 1][gr], kz[i >> 1][gr]) : kz[i >> 1][gr], sum[gr], s[i]);
-                        s[i] = fmaf(ks[i >> 1][gr], acc[gr][i] * unit[gr], s[i]);
+                        s[i] = fmaf((kWide ? fmaf(8.f, ks[i >> 1][gr], kz[i >> 1][gr]) : kz[i >> 1][gr]) * unit[gr], sum[gr], s[i]);
+                        s[i] = fmaf(ks[i >> 1][gr] * unit[gr], acc[gr][i], s[i]);
                     }
                 }
             } else {

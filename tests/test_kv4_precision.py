@@ -206,7 +206,7 @@ def test_a_missing_page_reaches_the_queries_that_see_it_and_no_other(cuda_device
 @pytest.mark.parametrize("d,hq,tokens", [(128, 8, 1), (256, 3, 1), (128, 2, 5)])
 def test_groups_of_a_query_may_be_of_any_size(cuda_device, dtype, d, hq, tokens):
     """One group of the keys is large where the queries are small, and another the other way round, so that both count in the scores."""
-    for a in (3, 8, 12, 13) if dtype is torch.float16 else (4, 10, 15, 30, 50):
+    for a in (3, 8, 12, 13) if dtype is torch.float16 else (4, 10, 15, 30, 50, 63, 90, 110):
         s = Server(cuda_device, dtype, d, 1, 32, [90, 17])
         gen = torch.Generator().manual_seed(a)
         k, v = (torch.randn(107, 1, d, generator=gen).clamp(-3, 3) for _ in range(2))
